@@ -1,0 +1,603 @@
+// Attention of query rows against the paged KV cache held in 8 bits
+// (fa_fwd_kvcache8): one token per sequence, a few, or chunks, batched or packed.
+// The cache's layout and scales are described in fa_kv8.h.
+//
+// kv8_split_kernel.  A workgroup owns up to 32 query rows of one sequence and
+// K/V head (row r is query r / group of query head r % group, so the heads that
+// share K/V share its bytes) and a split of the keys; its four waves take
+// 32-key tiles in turn, without a barrier, and merge at the end.  The rest is
+// as in decode_kernel (fa_decode.hip): S^T = K Q^T and O^T += V^T P^T on
+// v_mfma_f32_32x32x16, one query row per lane, fp32 maximum, sum and output.
+// What the 8 bits change:
+//  * K and V tiles go global -> LDS as they are, by LDS-DMA into a ring of the
+//    wave's own, and become 16-bit operands on the way from LDS to the matrix
+//    core: v_cvt_scalef32_pk takes the block's power-of-two scale with it, so a
+//    key's number times its scale is exact in bf16 (and in fp16 within its
+//    range) and no score or probability is rescaled.  LDS holds and moves
+//    half of what 16-bit tiles would.
+//  * A K row is read 16 bytes at a time: lane half g gets dims 32j + 16g ..,
+//    the low 8 for product 2j and the high 8 for product 2j + 1, and Q is laid
+//    out alike.  V^T comes from ds_read_b64_tr_b8: within 16 lanes, lanes 2r
+//    and 2r + 1 name the 16 bytes of row r and lane i receives column i of the
+//    8 rows, here the 8 keys whose probabilities the lane holds.
+//  * Page numbers and scales of all of a wave's tiles are loaded at the start,
+//    one lane per 16-key group, and handed to the scalar side by v_readlane:
+//    in the loop nothing but the tile loads counts on the vector-memory
+//    counter, so each wait names the tile it needs.
+// Keys past the sequence's end are never read: their bytes and scales may be
+// anything.  Where the mask differs between the rows of a tile, a V number that
+// is not finite would reach rows that do not see its key (0 * NaN); such tiles
+// are looked through, and one that holds any adds those per row and column
+// with a product of indicators.
+#pragma once
+
+#include "fa_common.h"
+#include "fa_kv8.h"
+
+namespace fa {
+
+constexpr int kKv8Waves = 4;
+constexpr int kKv8BN = 32;            // keys of a tile
+constexpr int kKv8MaxSplit = 32 * kKv8Waves * kKv8BN;   // 64 lanes hold the groups of 32 tiles per wave
+
+// The 8-bit types.  bad(): the high bit of each byte of a word whose number is
+// not finite.
+struct E4M3 {
+  template <class T>
+  __device__ static inline uint32_t cvt(uint32_t w, float scale, bool hi);
+  __device__ static inline uint32_t bad(uint32_t w) {
+    return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  }
+};
+struct E5M2 {
+  template <class T>
+  __device__ static inline uint32_t cvt(uint32_t w, float scale, bool hi);
+  __device__ static inline uint32_t bad(uint32_t w) {
+    return ((w & 0x7c7c7c7cu) + 0x04040404u) & 0x80808080u;
+  }
+};
+template <>
+__device__ inline uint32_t E4M3::cvt<F16>(uint32_t w, float s, bool hi) {
+  return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true))
+            : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false));
+}
+template <>
+__device__ inline uint32_t E4M3::cvt<BF16>(uint32_t w, float s, bool hi) {
+  return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true))
+            : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
+}
+template <>
+__device__ inline uint32_t E5M2::cvt<F16>(uint32_t w, float s, bool hi) {
+  return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, s, true))
+            : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, s, false));
+}
+template <>
+__device__ inline uint32_t E5M2::cvt<BF16>(uint32_t w, float s, bool hi) {
+  return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, s, true))
+            : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, s, false));
+}
+
+// Eight 8-bit numbers as a 16-bit MFMA operand.
+template <class T, class F8>
+__device__ inline u32x4 kv8_operand(uint32_t w0, uint32_t w1, float scale) {
+  return u32x4{F8::template cvt<T>(w0, scale, false), F8::template cvt<T>(w0, scale, true),
+               F8::template cvt<T>(w1, scale, false), F8::template cvt<T>(w1, scale, true)};
+}
+
+typedef int i32x2v __attribute__((__vector_size__(2 * sizeof(int))));
+__device__ inline u32x2 lds_read_tr8(const uint8_t* p) {
+  typedef __attribute__((address_space(3))) i32x2v lds_i32x2;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)p));
+}
+
+// Where the 16-byte chunk c of row r of a tile sits in its LDS row: such that
+// the 16 rows of a K read (one chunk each) and the 8 rows of a transposed V
+// read (keys 0..3 and 8..11 of a 16-key step, two chunks each) touch distinct
+// banks (256 bytes).
+template <int D>
+__device__ inline int kv8_k_chunk(int r, int c) {
+  constexpr int kRowsPer = 256 / D;
+  return c ^ ((r / kRowsPer) & (D / 16 - 1));
+}
+template <int D>
+__device__ inline int kv8_v_chunk(int r, int c) {
+  if constexpr (D == 256) return c ^ (((r & 3) | ((r >> 1) & 4)) << 1);
+  else if constexpr (D == 128) return c ^ ((((r >> 1) & 1) | ((r >> 2) & 2)) << 1);
+  else return c ^ (((r >> 3) & 1) << 1);
+}
+
+// The rows of a workgroup and the keys its sequence shows them.
+struct Kv8Rows {
+  int b, n;            // sequence, its queries
+  int64_t q0;          // its first row of q (packed), 0 otherwise
+  int L;               // its cached keys, clamped to [0, max_keys]
+};
+__device__ inline Kv8Rows kv8_rows(const Kv8AttnParams& p, int b) {
+  Kv8Rows s;
+  s.b = b;
+  s.q0 = 0;
+  s.n = p.seqlen_q;
+  if (p.cu_q != nullptr) {
+    // Offsets outside q would be read and written: an empty sequence instead.
+    const int64_t a = p.cu_q[b], e = p.cu_q[b + 1];
+    const bool ok = a >= 0 && e >= a && e <= p.total_q;
+    s.q0 = ok ? a : 0;
+    s.n = ok ? (int)min(e - a, (int64_t)p.seqlen_q) : 0;
+  }
+  const int L = p.seqlens != nullptr ? p.seqlens[b] : p.max_keys;
+  s.L = L < 0 ? 0 : L > p.max_keys ? p.max_keys : L;
+  return s;
+}
+// Row of the partials (and of the packed output) of query i.
+__device__ inline int64_t kv8_out_row(const Kv8AttnParams& p, const Kv8Rows& s, int i) {
+  return p.cu_q != nullptr ? s.q0 + i : (int64_t)s.b * p.seqlen_q + i;
+}
+__device__ inline int64_t kv8_base(const Kv8AttnParams& p, const Kv8Rows& s, int64_t sb, int64_t ss) {
+  return p.cu_q != nullptr ? s.q0 * ss : (int64_t)s.b * sb;
+}
+
+// Keys [lo, hi) that rows q_first .. q_last (queries) of a sequence see between
+// them.
+__device__ inline void kv8_key_range(const Kv8AttnParams& p, const Kv8Rows& s, int q_first, int q_last,
+                                     int& lo, int& hi) {
+  const int off = p.causal ? s.L - s.n : 0;
+  lo = 0;
+  hi = s.L;
+  if (p.causal) hi = min(hi, off + q_last + 1);
+  if (p.window_right >= 0) hi = min(hi, off + q_last + p.window_right + 1);
+  if (p.window_left >= 0) lo = max(lo, off + q_first - p.window_left);
+  hi = max(hi, 0);
+}
+
+template <int D, int NST>
+struct Kv8Tile {
+  static constexpr int kBytes = kKv8BN * D;            // one tile of K or V
+  static constexpr int kRing = NST * 2 * kBytes;       // per wave
+  static constexpr int kMerge = 32 * (D + 2) * 4;      // per wave: O rows and (m, l)
+  static constexpr int kLds = kKv8Waves * (kRing > kMerge ? kRing : kMerge);
+};
+
+template <class T, class F8, int D, int NST, bool GENERIC>
+__global__ __launch_bounds__(kKv8Waves * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+void kv8_split_kernel(const Kv8AttnParams p) {
+  using Tile = Kv8Tile<D, NST>;
+  constexpr int BN = kKv8BN;
+  constexpr int CPR = D / 16;              // 16-byte chunks of a row
+  constexpr int RPI = 64 / CPR;            // rows of one DMA instruction
+  constexpr int NI = BN / RPI;             // DMA instructions of a tile
+  constexpr int IPG = 16 / RPI;            // of a 16-key group
+  constexpr int NDB = D / 32;
+  static_assert(RPI <= 16 && 16 % RPI == 0, "an instruction stays within a 16-key group");
+
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem8[];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c32 = lane & 31;
+  const int g = lane >> 5;
+
+  // K/V heads vary fastest, the split slowest: as in decode_kernel.
+  int id = blockIdx.x;
+  const int kvh = id % p.heads_k;
+  id /= p.heads_k;
+  const int rb = id % p.row_blocks;
+  id /= p.row_blocks;
+  const int b = id % p.batch;
+  const int split = id / p.batch;
+
+  const Kv8Rows s = kv8_rows(p, b);
+  const int G = (int)p.group.d;
+  const int rows = min(s.n * G - rb * 32, 32);
+  if (rows <= 0) return;
+  const int q_first = (int)fdiv(rb * 32, p.group), q_last = (int)fdiv(rb * 32 + rows - 1, p.group);
+  int lo, hi;
+  kv8_key_range(p, s, q_first, q_last, lo, hi);
+  // This split's keys.  Split 0 always runs, so that rows without keys are
+  // written when there is no combine.
+  const int k_begin = max(split * p.split_keys, lo & ~(BN - 1));
+  const int k_end = min(hi, (split + 1) * p.split_keys);
+  if (k_begin >= k_end && split > 0) return;
+
+  const int r = min(c32, rows - 1);
+  const bool row_valid = c32 < rows;
+  const int qi = (int)fdiv(rb * 32 + r, p.group);
+  const int head = kvh * G + (rb * 32 + r - qi * G);
+  const int off = p.causal ? s.L - s.n : 0;
+  const int qpos = qi + off;
+  int key_hi = s.L - 1, key_lo = 0;
+  if (p.causal) key_hi = min(key_hi, qpos);
+  if (p.window_right >= 0) key_hi = min(key_hi, qpos + p.window_right);
+  if (p.window_left >= 0) key_lo = max(0, qpos - p.window_left);
+  // Keys that every row sees: tiles within need no mask.
+  int all_lo = 0, all_hi = s.L - 1;
+  if (p.causal) all_hi = min(all_hi, q_first + off);
+  if (p.window_right >= 0) all_hi = min(all_hi, q_first + off + p.window_right);
+  if (p.window_left >= 0) all_lo = max(0, q_last + off - p.window_left);
+  float slope = 0.f;
+  if (GENERIC && p.alibi != nullptr) slope = p.alibi[(int64_t)b * p.alibi_sb + head];
+
+  // Q^T in the order of the K operand (rows past the last repeat it).
+  u32x4 qreg[2 * NDB];
+  {
+    const uint16_t* qrow = static_cast<const uint16_t*>(p.q) + kv8_base(p, s, p.q_sb, p.q_ss) +
+                           (int64_t)qi * p.q_ss + (int64_t)head * p.q_sh;
+#pragma unroll
+    for (int j = 0; j < NDB; ++j) {
+      qreg[2 * j] = load16(qrow + 32 * j + 16 * g);
+      qreg[2 * j + 1] = load16(qrow + 32 * j + 16 * g + 8);
+    }
+  }
+
+  // Lane i holds page, slot and scales of 16-key group i % 2 of this wave's tile
+  // i / 2.  A group without keys names no page; its scale is 1.
+  const int n_tiles = k_end > k_begin ? (k_end - k_begin + BN - 1) / BN : 0;
+  const int my_tiles = (n_tiles - w + kKv8Waves - 1) / kKv8Waves;
+  int page_l = -1, slot_l = 0;
+  uint32_t ks_l = 127u << 23, vs_l = 127u << 23;
+  {
+    const int key = k_begin + (w + (lane >> 1) * kKv8Waves) * BN + (lane & 1) * 16;
+    if (key < k_end) {
+      const int col = (int)fdiv(key, p.page);
+      slot_l = key - col * (int)p.page.d;
+      page_l = p.table != nullptr ? p.table[(int64_t)b * p.table_stride + col] : b;
+      if (page_l < 0 || page_l >= p.num_pages) {
+        page_l = -1;
+      } else {
+        const int blk = slot_l >> p.log2_block;
+        ks_l = (uint32_t)p.ks[page_l * p.ks_sp + blk * p.ks_sb + kvh * p.ks_sh] << 23;
+        vs_l = (uint32_t)p.vs[page_l * p.vs_sp + blk * p.vs_sb + kvh * p.vs_sh] << 23;
+      }
+    }
+  }
+
+  uint8_t* ring = smem8 + w * Tile::kRing;
+  const uint32_t ring_lds = lds_address(ring);
+  // LDS-DMA of tile t (of this wave) into its stage.  Lane l of instruction m
+  // fills chunk position l % CPR of row m * RPI + l / CPR.
+  auto issue = [&](int t) {
+    const int key0 = k_begin + (w + t * kKv8Waves) * BN;
+    const uint32_t st = ring_lds + (uint32_t)((t % NST) * 2 * Tile::kBytes);
+    const int row_l = lane / CPR, pos = lane % CPR;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const int64_t sp = kv ? p.v_sp : p.k_sp, ss = kv ? p.v_ss : p.k_ss, sh = kv ? p.v_sh : p.k_sh;
+      const uint8_t* base = kv ? p.v : p.k;
+#pragma unroll
+      for (int gr = 0; gr < 2; ++gr) {
+        // (tiles past the last get an empty resource, so that the count of
+        // loads in flight is the same on every path)
+        const int at = min(2 * t + gr, 63);
+        const int page = t < my_tiles ? __builtin_amdgcn_readlane(page_l, at) : -1;
+        const int slot = __builtin_amdgcn_readlane(slot_l, at);
+        const int left = min(s.L - (key0 + 16 * gr), 16);
+        const bool live = page >= 0 && left > 0;
+        const u32x4 rs = make_rsrc_words(live ? base + page * sp + slot * ss + kvh * sh : base,
+                                         live ? (uint32_t)((left - 1) * ss + D) : 0u);
+#pragma unroll
+        for (int m = gr * IPG; m < (gr + 1) * IPG; ++m) {
+          const int row = m * RPI + row_l;
+          const int chunk = kv ? kv8_v_chunk<D>(row, pos) : kv8_k_chunk<D>(row, pos);
+          buf_load16_lds(rs, st + (uint32_t)(kv * Tile::kBytes + m * 1024),
+                         (uint32_t)((row - 16 * gr) * (int)ss + chunk * 16));
+        }
+      }
+    }
+  };
+
+  f32x16 acc[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) acc[db] = f32x16{};
+  float m_run = -INFINITY, l_run = 0.f;
+  const float sl = GENERIC ? kLog2e : p.scale * kLog2e;
+
+  for (int t = 0; t < NST - 1; ++t) issue(t);
+  // The compiler does not count the LDS-DMA loads: a use of a loaded register
+  // inside the loop would wait there for everything in flight, so all of them
+  // are waited for here, once.
+#pragma unroll
+  for (int j = 0; j < 2 * NDB; ++j) asm volatile("" : "+v"(qreg[j]));
+  asm volatile("" : "+v"(ks_l), "+v"(vs_l), "+v"(slope));
+  for (int t = 0; t < my_tiles; ++t) {
+    const int n0 = k_begin + (w + t * kKv8Waves) * BN;
+    // (this wave's LDS reads of the stage that is filled now ended with the
+    // previous tile's products)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    issue(t + NST - 1);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((NST - 1) * 2 * NI + NI));   // K of tile t
+    asm volatile("" ::: "memory");
+    const uint8_t* kt = ring + (t % NST) * 2 * Tile::kBytes;
+    const uint8_t* vt = kt + Tile::kBytes;
+
+    const float ks0 = __uint_as_float(__builtin_amdgcn_readlane(ks_l, 2 * t));
+    const float ks1 = __uint_as_float(__builtin_amdgcn_readlane(ks_l, 2 * t + 1));
+    const float ksc = c32 < 16 ? ks0 : ks1;
+    f32x16 sc = f32x16{};
+#pragma unroll
+    for (int j = 0; j < NDB; ++j) {
+      const u32x4 raw = load16(kt + c32 * D + kv8_k_chunk<D>(c32, 2 * j + g) * 16);
+      sc = T::mfma32(kv8_operand<T, F8>(raw[0], raw[1], ksc), qreg[2 * j], sc);
+      sc = T::mfma32(kv8_operand<T, F8>(raw[2], raw[3], ksc), qreg[2 * j + 1], sc);
+    }
+
+    const bool masked = n0 < all_lo || n0 + BN - 1 > all_hi;
+    float mx = -INFINITY;
+    if (GENERIC) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int key = n0 + 8 * (v >> 2) + 4 * g + (v & 3);
+        float x = sc[v] * p.scale;
+        if (p.alibi != nullptr) x = fmaf(-slope, fabsf((float)(qpos - key)), x);
+        if (p.softcap > 0.f) {
+          // softcap * tanh(x / softcap) = softcap * (1 - 2 / (exp(2 x / softcap) + 1))
+          const float ex = __builtin_amdgcn_exp2f(x * (2.f * kLog2e / p.softcap));
+          x = p.softcap * (1.f - 2.f / (ex + 1.f));
+        }
+        sc[v] = x;
+      }
+    }
+    if (masked) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int key = n0 + 8 * (v >> 2) + 4 * g + (v & 3);
+        if (key < key_lo || key > key_hi || key >= k_end) sc[v] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[v]);
+    mx = halves_max(mx) * sl;
+    const float m_new = fmaxf(m_run, mx);
+    if (__builtin_amdgcn_ballot_w64(m_new > m_run)) {
+      const float alpha = m_new == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) acc[db] *= alpha;
+      m_run = m_new;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    u32x4 pb[2];
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[cc * 8 + 2 * j], sl, -m_use));
+        const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[cc * 8 + 2 * j + 1], sl, -m_use));
+        pb[cc][j] = T::pack2(e0, e1);
+        l_run += e0 + e1;
+      }
+
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((NST - 1) * 2 * NI));   // V of tile t
+    asm volatile("" ::: "memory");
+    // The lane's 8 keys of step cc: 16 cc + 4 g + {0..3, 8..11}; row i / 2 of
+    // the transposed read, i the lane among its 16.
+    const int vr = (lane & 15) >> 1, vkey = 4 * g + (vr & 3) + 8 * (vr >> 2);
+    const int vc = ((lane >> 4) & 1), vh = 8 * (lane & 1);
+    uint32_t flags = 0;
+    u32x2 raw[2][NDB];
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        const int row = 16 * cc + vkey;
+        raw[cc][db] = lds_read_tr8(vt + row * D + kv8_v_chunk<D>(row, 2 * db + vc) * 16 + vh);
+      }
+    const bool mixed = n0 < all_lo || (n0 + BN - 1 > all_hi && all_hi < s.L - 1);
+    if (mixed) {
+#pragma unroll
+      for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) flags |= F8::bad(raw[cc][db][0]) | F8::bad(raw[cc][db][1]);
+    }
+    const bool dirty = mixed && __builtin_amdgcn_ballot_w64(flags != 0) != 0;
+    if (dirty) {
+      // Visible (key, row) pairs and numbers that are not finite, as 1 and 0: a
+      // row gets NaN in the columns where their product is not zero.
+      u32x4 seen[2];
+#pragma unroll
+      for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          seen[cc][j] = T::pack2(sc[cc * 8 + 2 * j] == -INFINITY ? 0.f : 1.f,
+                                 sc[cc * 8 + 2 * j + 1] == -INFINITY ? 0.f : 1.f);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        f32x16 hit = f32x16{};
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          u32x4 ind;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t f = F8::bad(raw[cc][db][e]);
+            ind[2 * e] = T::pack2((f & 0x80u) ? 1.f : 0.f, (f & 0x8000u) ? 1.f : 0.f);
+            ind[2 * e + 1] = T::pack2((f & 0x800000u) ? 1.f : 0.f, (f & 0x80000000u) ? 1.f : 0.f);
+            raw[cc][db][e] &= ~((f >> 7) * 0xffu);
+          }
+          hit = T::mfma32(ind, seen[cc], hit);
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (hit[v] > 0.f) acc[db][v] = __uint_as_float(0x7fc00000u);
+      }
+    }
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc) {
+      const float vsc = __uint_as_float(__builtin_amdgcn_readlane(vs_l, 2 * t + cc));
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+        acc[db] = T::mfma32(kv8_operand<T, F8>(raw[cc][db][0], raw[cc][db][1], vsc), pb[cc], acc[db]);
+    }
+  }
+
+  // ------------------------------------------------------------ merge waves
+  // The rings become the rows' merge area once every load into them has landed
+  // and every wave is done reading.
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  asm volatile("" ::: "memory");
+  __syncthreads();
+  float* mo = reinterpret_cast<float*>(smem8);
+  float* ml = mo + kKv8Waves * 32 * D;
+  const float l_w = halves_sum(l_run);
+  if (row_valid) {
+    float* orow = mo + (w * 32 + c32) * D;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        *reinterpret_cast<f32x4*>(orow + db * 32 + 8 * q4 + 4 * g) =
+            f32x4{acc[db][4 * q4], acc[db][4 * q4 + 1], acc[db][4 * q4 + 2], acc[db][4 * q4 + 3]};
+    if (g == 0) {
+      ml[(w * 32 + c32) * 2] = m_run;
+      ml[(w * 32 + c32) * 2 + 1] = l_w;
+    }
+  }
+  __syncthreads();
+  // Thread t: row t / 8, D / 8 dims from D / 8 * (t % 8).
+  constexpr int DPT = D / 8;
+  const int rr = tid >> 3;
+  if (rr >= rows) return;
+  const int d0 = (tid & 7) * DPT;
+  float M = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < kKv8Waves; ++u) M = fmaxf(M, ml[(u * 32 + rr) * 2]);
+  float total = 0.f, wt[kKv8Waves];
+#pragma unroll
+  for (int u = 0; u < kKv8Waves; ++u) {
+    // (a wave without keys has l = 0; a NaN sum stays one)
+    const float l = ml[(u * 32 + rr) * 2 + 1];
+    wt[u] = l != 0.f ? __builtin_amdgcn_exp2f(ml[(u * 32 + rr) * 2] - M) : 0.f;
+    total += l * wt[u];
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  float o[DPT];
+#pragma unroll
+  for (int e = 0; e < DPT; ++e) o[e] = 0.f;
+#pragma unroll
+  for (int u = 0; u < kKv8Waves; ++u) {
+    const float* src = mo + (u * 32 + rr) * D + d0;
+#pragma unroll
+    for (int e = 0; e < DPT; e += 4) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(src + e);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[e + k] = fmaf(x[k], wt[u], o[e + k]);
+    }
+  }
+  const int oi = (int)fdiv(rb * 32 + rr, p.group);
+  const int oh = kvh * G + (rb * 32 + rr - oi * G);
+  if (p.num_splits == 1) {
+    uint16_t* dst = static_cast<uint16_t*>(p.o) + kv8_base(p, s, p.o_sb, p.o_ss) +
+                    (int64_t)oi * p.o_ss + (int64_t)oh * p.o_sh + d0;
+#pragma unroll
+    for (int e = 0; e < DPT; e += 8) {
+      u32x4 val;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) val[k] = T::pack2(o[e + 2 * k] * inv, o[e + 2 * k + 1] * inv);
+      store16(dst + e, val);
+    }
+  } else {
+    const int64_t prow = ((int64_t)split * p.total_q + kv8_out_row(p, s, oi)) * p.heads_q + oh;
+    float* dst = p.o_part + prow * D + d0;
+#pragma unroll
+    for (int e = 0; e < DPT; e += 4)
+      *reinterpret_cast<f32x4*>(dst + e) = f32x4{o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
+    if ((tid & 7) == 0)
+      p.lse_part[prow] = total == 0.f ? -INFINITY : M + __log2f(total);
+  }
+}
+
+// Merges the splits of each row: out = sum_s 2^(lse_s - lse) o_s over the
+// splits that hold keys its workgroup saw (the others are unwritten).  One
+// thread per row and 4 dims, a workgroup within one sequence; partials are
+// fetched in batches of independent loads.
+template <class T, int D>
+__global__ __launch_bounds__(256) void kv8_combine_kernel(const Kv8AttnParams p) {
+  constexpr int kBatch = 8;
+  constexpr int kQuads = D / 4;
+  const int b = blockIdx.y;
+  const Kv8Rows s = kv8_rows(p, b);
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t item = idx / kQuads;
+  if (item >= (int64_t)s.n * p.heads_q) return;
+  const int qd = (int)(idx % kQuads), h = (int)(item % p.heads_q), i = (int)(item / p.heads_q);
+  const int G = (int)p.group.d;
+  // The splits that the row's 32-row block ran: those that meet its keys.
+  const int rb = (i * G + h % G) / 32, last = min(rb * 32 + 31, s.n * G - 1);
+  int lo, hi;
+  kv8_key_range(p, s, (int)fdiv(rb * 32, p.group), (int)fdiv(last, p.group), lo, hi);
+  const int s_lo = lo / p.split_keys;
+  const int n = hi > lo ? min(p.num_splits, (hi + p.split_keys - 1) / p.split_keys) : 0;
+  const int64_t row = kv8_out_row(p, s, i) * p.heads_q + h, step = p.total_q * p.heads_q;
+  float m = -INFINITY, tot = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  bool bad = false;
+  for (int s0 = s_lo; s0 < n; s0 += kBatch) {
+    float ls[kBatch];
+    f32x4 o[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const bool on = s0 + u < n;
+      ls[u] = on ? p.lse_part[(s0 + u) * step + row] : -INFINITY;
+      o[u] = on ? *reinterpret_cast<const f32x4*>(p.o_part + ((s0 + u) * step + row) * D + qd * 4)
+                : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float mb = m;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      mb = fmaxf(mb, ls[u]);
+      bad |= ls[u] != ls[u];
+    }
+    if (mb == -INFINITY) continue;
+    const float again = __builtin_amdgcn_exp2f(m - mb);   // m == -inf -> 0
+    tot *= again;
+    acc *= again;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const float wgt = ls[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ls[u] - mb);
+      tot += wgt;
+      acc += wgt * o[u];
+    }
+    m = mb;
+  }
+  const float inv = bad ? __uint_as_float(0x7fc00000u) : tot > 0.f ? 1.f / tot : 0.f;
+  uint16_t* dst = static_cast<uint16_t*>(p.o) + kv8_base(p, s, p.o_sb, p.o_ss) + (int64_t)i * p.o_ss +
+                  (int64_t)h * p.o_sh + qd * 4;
+  u32x2 val;
+  val[0] = T::pack2(acc[0] * inv, acc[1] * inv);
+  val[1] = T::pack2(acc[2] * inv, acc[3] * inv);
+  *reinterpret_cast<u32x2*>(dst) = val;
+}
+
+template <class T, class F8, int D, bool GENERIC>
+hipError_t launch_kv8_split(const Kv8AttnParams& p, hipStream_t st) {
+  constexpr int NST = D == 256 ? 2 : D == 128 ? 2 : 4;
+  using Tile = Kv8Tile<D, NST>;
+  auto kern = kv8_split_kernel<T, F8, D, NST, GENERIC>;
+  static std::atomic<uint64_t> lds_devices{0};
+  if (hipError_t e = set_lds_limit(lds_devices, kern, Tile::kLds); e != hipSuccess) return e;
+  const int64_t wgs = (int64_t)p.num_splits * p.batch * p.row_blocks * p.heads_k;
+  if (wgs <= 0) return hipSuccess;
+  if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(kKv8Waves * 64), Tile::kLds, st, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.num_splits == 1) return e;
+  const int64_t threads = (int64_t)p.seqlen_q * p.heads_q * (D / 4);
+  hipLaunchKernelGGL((kv8_combine_kernel<T, D>), dim3((unsigned)((threads + 255) / 256), (unsigned)p.batch),
+                     dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_kv8_attn(int store, const Kv8AttnParams& p, int head_dim, hipStream_t st) {
+  const bool generic = p.alibi != nullptr || p.softcap > 0.f || !(p.scale > 0.f);
+#define FA_KV8(FF, DD)                                                     \
+  return generic ? launch_kv8_split<T, FF, DD, true>(p, st) : launch_kv8_split<T, FF, DD, false>(p, st);
+#define FA_KV8_D(FF)                      \
+  if (head_dim == 64) { FA_KV8(FF, 64) }   \
+  if (head_dim == 128) { FA_KV8(FF, 128) } \
+  if (head_dim == 256) { FA_KV8(FF, 256) }
+  if (store == 0) { FA_KV8_D(E4M3) } else { FA_KV8_D(E5M2) }
+#undef FA_KV8_D
+#undef FA_KV8
+  return hipErrorInvalidValue;
+}
+
+}  // namespace fa

@@ -20,3 +20,10 @@ from flash_attn_triton.flash_attn_interface import (
     flash_attn_varlen_qkvpacked_func as flash_attn_unpadded_qkvpacked_func,
     flash_attn_varlen_kvpacked_func as flash_attn_unpadded_kvpacked_func,
 )
+
+# Serving over a KV cache held in 8 bits.
+from flash_attn_triton.kvcache_8bit import (
+    flash_attn_with_kvcache_8bit,
+    kvcache_append_8bit,
+    paged_kvcache_slots,
+)

@@ -21,3 +21,9 @@ from .flash_attn_interface import (
     FlashSelfAttention,
     FlashCrossAttention,
 )
+
+from .kvcache_8bit import (
+    flash_attn_with_kvcache_8bit,
+    kvcache_append_8bit,
+    paged_kvcache_slots,
+)

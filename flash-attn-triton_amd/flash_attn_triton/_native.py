@@ -29,6 +29,8 @@ FA_ERR_HIP = 3
 FA_DTYPE_F16 = 0
 FA_DTYPE_BF16 = 1
 FA_DTYPE_F32 = 2
+FA_STORE_E4M3 = 0
+FA_STORE_E5M2 = 1
 
 _i64 = ctypes.c_int64
 _u64 = ctypes.c_uint64
@@ -86,6 +88,15 @@ _SIGNATURES = {
     "fa_check_ranges": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "fa_check_bounds": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "fa_check_wait": (_int, [_vp, _int, _vp]),
+    "fa_kvcache_slots": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp,
+                                _vp, _vp, _vp, _vp]),
+    "fa_kvcache8_append": (_int, [_vp, _vp, _i64p, _i64p, _int, _vp, _vp, _i64p, _i64p, _int, _vp, _vp,
+                                  _i64p, _i64p, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "fa_fwd_kvcache8_plan": (_int, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32p, _i64p]),
+    "fa_fwd_kvcache8": (_int, [_vp, _vp, _i64p, _i64p, _int, _vp, _vp, _i64p, _i64p, _int, _vp, _vp,
+                               _i64p, _i64p, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64,
+                               _i64, _i64, _i64, _i64, _i64, _f32, _int, _i64, _i64, _f32, _vp, _i64,
+                               _i32, _vp, _i64, _vp]),
     "fa_quant_k_int8": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64p, _vp]),
     "fa_fwd_int8": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64p, _i64p,
                            _i64p, _f32, _int, _i64, _i64, _vp]),
@@ -452,6 +463,74 @@ def kvcache_update(k_new, v_new, k_cache, v_cache, cache_seqlens, block_table, c
         Sq, Hq, _ptr(lens_out), B, n, heads_k, D, *st, dtype_code(q.dtype), _ptr(guard),
         0 if guard is None else guard.numel(), _stream(q.device))
     _check(status, "fa_kvcache_update")
+
+
+def store_code(dtype: torch.dtype) -> int:
+    if dtype == torch.float8_e4m3fn:
+        return FA_STORE_E4M3
+    if dtype == torch.float8_e5m2:
+        return FA_STORE_E5M2
+    raise RuntimeError(f"flash_attn_triton: an 8-bit cache is float8_e4m3fn or float8_e5m2, not {dtype}")
+
+
+def kvcache_slots(block_table, cache_seqlens, new_seqlens, free_pages, free_start, page_size: int,
+                  slot_mapping, positions, cu_seqlens, seqlens_out, free_end) -> None:
+    """Pages and slots of the next tokens from the lengths (see fa_kvcache_slots)."""
+    status = load().fa_kvcache_slots(
+        _ptr(block_table), block_table.stride(0), block_table.shape[1], _ptr(cache_seqlens),
+        _ptr(new_seqlens), cache_seqlens.numel(), _ptr(free_pages), free_pages.numel(), _ptr(free_start),
+        page_size, slot_mapping.numel(), _ptr(slot_mapping), _ptr(positions), _ptr(cu_seqlens),
+        _ptr(seqlens_out), _ptr(free_end), _stream(block_table.device))
+    _check(status, "fa_kvcache_slots")
+
+
+def kvcache8_append(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapping) -> None:
+    """Quantize k / v [T, Hk, D] into the 8-bit cache (see fa_kvcache8_append)."""
+    T, Hk, D = k.shape
+    pages, page = k_cache.shape[:2]
+    status = load().fa_kvcache8_append(
+        _ptr(k), _ptr(v), _strides(k.stride()[:2]), _strides(v.stride()[:2]), dtype_code(k.dtype),
+        _ptr(k_cache), _ptr(v_cache), _strides(k_cache.stride()[:3]), _strides(v_cache.stride()[:3]),
+        store_code(k_cache.dtype), _ptr(k_scale), _ptr(v_scale), _strides(k_scale.stride()),
+        _strides(v_scale.stride()), _ptr(slot_mapping), T, pages, page, page // k_scale.shape[1], Hk, D,
+        _stream(k.device))
+    _check(status, "fa_kvcache8_append")
+
+
+@functools.lru_cache(maxsize=1024)
+def kvcache8_plan(batch: int, max_seqlen_q: int, total_q: int, heads_q: int, heads_k: int, head_dim: int,
+                  max_keys: int):
+    splits, ws = ctypes.c_int32(0), ctypes.c_int64(0)
+    _check(load().fa_fwd_kvcache8_plan(batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys,
+                                       ctypes.byref(splits), ctypes.byref(ws)), "fa_fwd_kvcache8_plan")
+    return int(splits.value), int(ws.value)
+
+
+def fwd_kvcache8(q, out, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, cu_seqlens_q,
+                 batch: int, max_seqlen_q: int, max_keys: int, softmax_scale: float, causal: bool,
+                 window_left: int, window_right: int, softcap: float, alibi) -> None:
+    """Attention of q [B, Sq, Hq, D], or packed [T, Hq, D] with cu_seqlens_q, against
+    the 8-bit cache (see fa_fwd_kvcache8)."""
+    Hq, D = q.shape[-2:]
+    pages, page, Hk = k_cache.shape[:3]
+    packed = cu_seqlens_q is not None
+    total = q.shape[0] if packed else batch * max_seqlen_q
+    splits, ws_bytes = kvcache8_plan(batch, max_seqlen_q, total, Hq, Hk, D, max_keys)
+    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    qs, os_ = q.stride(), out.stride()
+    q_stride = _strides((0,) + qs[:2] if packed else qs[:3])
+    o_stride = _strides((0,) + os_[:2] if packed else os_[:3])
+    tabled = block_table is not None
+    status = load().fa_fwd_kvcache8(
+        _ptr(q), _ptr(out), q_stride, o_stride, dtype_code(q.dtype), _ptr(k_cache), _ptr(v_cache),
+        _strides(k_cache.stride()[:3]), _strides(v_cache.stride()[:3]), store_code(k_cache.dtype),
+        _ptr(k_scale), _ptr(v_scale), _strides(k_scale.stride()), _strides(v_scale.stride()),
+        _ptr(cache_seqlens), _ptr(block_table), block_table.stride(0) if tabled else 0,
+        block_table.shape[1] if tabled else 0, pages, page, page // k_scale.shape[1], _ptr(cu_seqlens_q),
+        batch, max_seqlen_q, total, max_keys, Hq, Hk, D, softmax_scale, int(bool(causal)), window_left,
+        window_right, softcap, _ptr(alibi), alibi.stride(0) if alibi is not None else 0, splits,
+        _ptr(workspace), ws_bytes, _stream(q.device))
+    _check(status, "fa_fwd_kvcache8")
 
 
 def quant_k_int8(k, k8, s_k) -> None:

@@ -415,6 +415,90 @@ int fa_check_bounds(int n, const void* const* a, const int* a_bytes, const void*
  * written.  Fails if the stream fails, or drains without them. */
 int fa_check_wait(const int64_t* result, int n, fa_stream_t stream);
 
+/* The paged KV cache in 8 bits.  k_cache / v_cache are [num_pages, page_size,
+ * heads_k, head_dim] of an 8-bit floating-point type (FA_STORE_*, OCP encodings)
+ * with a scale byte per block of `block` slots and head, [num_pages, page_size /
+ * block, heads_k]: a cached value is its number times 2^(byte - 127).  block is
+ * a power of two of at least 16 that divides page_size; head_dim is 64, 128 or
+ * 256.  Cache strides are {page, slot, head} in bytes, scale strides {page,
+ * block, head}; rows are 16-byte aligned.  A batched cache is one whose pages
+ * are its rows. */
+#define FA_STORE_E4M3 0
+#define FA_STORE_E5M2 1
+
+/* Pages and slots of the next tokens of `batch` requests, on the device from
+ * their lengths (the bookkeeping that a host otherwise does between the steps
+ * of a paged KV cache).  Request b holds cache_seqlens[b] tokens and gets
+ * new_seqlens[b]; the pages its new tokens begin are taken from free_pages
+ * (n_free numbers) from index free_start[0] on (NULL: 0), requests in order,
+ * and written into its row of block_table [batch, cols].  Row cu_seqlens[b] + i
+ * of the packed outputs is its new token i: positions (its index in the
+ * sequence) and slot_mapping (page * page_size + position % page_size).
+ * max_tokens is the number of packed rows; rows past the last request get slot
+ * -1 and position 0.  cu_seqlens [batch + 1] are the prefix sums of
+ * new_seqlens (at most max_tokens), seqlens_out the lengths afterwards and
+ * free_end[0] the index of the first free page left.  A request is refused
+ * (slots -1, its length and table row as they were) if it passes the end of
+ * its table row or of the packed rows, or if it needs pages and those needed
+ * up to and with it are more than are free.  Lengths below 0 count as 0.
+ * Nothing is read or written outside the arrays whatever they hold. */
+int fa_kvcache_slots(int32_t* block_table, int64_t block_table_stride, int64_t cols,
+                     const int32_t* cache_seqlens, const int32_t* new_seqlens, int64_t batch,
+                     const int32_t* free_pages, int64_t n_free, const int32_t* free_start,
+                     int64_t page_size, int64_t max_tokens, int64_t* slot_mapping, int32_t* positions,
+                     int32_t* cu_seqlens, int32_t* seqlens_out, int32_t* free_end,
+                     fa_stream_t stream);
+
+/* New rows k / v [tokens, heads_k, head_dim] (`dtype`, strides {row, head})
+ * quantized into the 8-bit cache, row t to slot slot_mapping[t] (page *
+ * page_size + slot in the page; a slot outside the cache is skipped).  The rows
+ * of one scale block are a run: consecutive rows for consecutive slots.  A run
+ * that begins at its block's first slot sets the block's scale to the least
+ * that holds its finite numbers; another one raises it where that is needed,
+ * and then rounds the slots below the run, which the block holds already, to
+ * the new scale.  Rounding is to nearest even; a number that is not finite
+ * becomes NaN.  Two runs of one call must not fall into the same block. */
+int fa_kvcache8_append(const void* k, const void* v, const int64_t* k_stride, const int64_t* v_stride,
+                       int dtype, void* k_cache, void* v_cache, const int64_t* k_cache_stride,
+                       const int64_t* v_cache_stride, int store, uint8_t* k_scale, uint8_t* v_scale,
+                       const int64_t* k_scale_stride, const int64_t* v_scale_stride,
+                       const int64_t* slot_mapping, int64_t tokens, int64_t num_pages,
+                       int64_t page_size, int64_t block, int64_t heads_k, int64_t head_dim,
+                       fa_stream_t stream);
+
+/* Splits of the keys and bytes of workspace (fp32 partial rows) of
+ * fa_fwd_kvcache8.  Host only. */
+int fa_fwd_kvcache8_plan(int64_t batch, int64_t max_seqlen_q, int64_t total_q, int64_t heads_q,
+                         int64_t heads_k, int64_t head_dim, int64_t max_keys, int32_t* num_splits,
+                         int64_t* workspace_bytes);
+
+/* Attention of queries against the 8-bit cache: fa_fwd_kvcache with q and out
+ * fp16 or bf16, [batch, max_seqlen_q, heads_q, head_dim] (strides {batch, query,
+ * head}), or, with cu_seqlens_q [batch + 1], packed [total_q, heads_q, head_dim]
+ * (the batch stride unused): sequence b has queries cu_seqlens_q[b] ..
+ * cu_seqlens_q[b + 1] - 1, at most max_seqlen_q of them.  Query i of n sits at
+ * position i + L_b - n when causal, else at i, L_b = cache_seqlens[b] (NULL:
+ * max_keys) clamped to [0, max_keys].  Keys are found through block_table
+ * [batch, block_table_cols], or in page b without one; max_keys is at most the
+ * table's or the page's slots.  A cached value counts as q's type holds it
+ * (exact in bf16; in fp16 within its range).  softcap, windows and slopes as in
+ * fa_fwd_varlen.  Rows of packed q outside every sequence are not written.
+ * Whatever the device arrays hold nothing outside the tensors is read or
+ * written: a page outside the cache reads as zeros, a sequence whose offsets
+ * leave q has no queries.  num_splits and workspace come from the plan. */
+int fa_fwd_kvcache8(const void* q, void* out, const int64_t* q_stride, const int64_t* o_stride, int dtype,
+                    const void* k_cache, const void* v_cache, const int64_t* k_cache_stride,
+                    const int64_t* v_cache_stride, int store, const uint8_t* k_scale,
+                    const uint8_t* v_scale, const int64_t* k_scale_stride,
+                    const int64_t* v_scale_stride, const int32_t* cache_seqlens,
+                    const int32_t* block_table, int64_t block_table_stride, int64_t block_table_cols,
+                    int64_t num_pages, int64_t page_size, int64_t block, const int32_t* cu_seqlens_q,
+                    int64_t batch, int64_t max_seqlen_q, int64_t total_q, int64_t max_keys,
+                    int64_t heads_q, int64_t heads_k, int64_t head_dim, float softmax_scale, int causal,
+                    int64_t window_left, int64_t window_right, float softcap, const float* alibi_slopes,
+                    int64_t alibi_batch_stride, int32_t num_splits, void* workspace,
+                    int64_t workspace_bytes, fa_stream_t stream);
+
 /* Per-token INT8 quantization of K (fp16), bit-exact with
  * `_quantize_k_rows` (attention_kernel_int8.py:58-79, launched at :232):
  *   s = fp32(max(amax_row, 1)) / 127;  k8 = round_half_away(fp32(k) * (1/s)).
