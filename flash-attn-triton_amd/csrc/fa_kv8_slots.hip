@@ -7,7 +7,7 @@
 // table[b][pos / page] * page + pos % page.  A request that does not fit its
 // table row or the packed rows, or whose prefix of page needs passes the free
 // pages (unless it needs none), gets no page: its slots are -1 and its length
-// stays.
+// stays.  The index handed back counts the needs up to the last request served.
 //
 // One launch without any exchange between workgroups: every workgroup forms
 // the prefix sums of the lengths itself, 4 KiB of LDS per 512 requests, and
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(kThreads) void kvcache_slots_kernel(const SlotsPara
         cu[b] = (int)min(r, (int64_t)p.rows);
         pages[b] = served ? (int)min(before, kIntMax) : -1;
         old_len[b] = o[i];
-        if (served && need[i] > 0) most = (int)upto;
+        if (served) most = (int)min(upto, kIntMax - start);
         if (blockIdx.x == 0) {
           p.cu[c0 + b] = (int)min(r, (int64_t)p.rows);
           p.seqlens[c0 + b] = served ? o[i] + a[i] : o[i];

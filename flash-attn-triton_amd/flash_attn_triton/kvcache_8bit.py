@@ -113,8 +113,8 @@ def paged_kvcache_slots(block_table, cache_seqlens, new_seqlens, free_pages, pag
         page_size: int. Tokens per page.
         max_tokens: int. Rows of the packed outputs, at least the sum of
             new_seqlens.
-        free_start: (1,) int32, index of the first page of free_pages that is
-            still free (None: 0); what a call returns goes into the next one.
+        free_start: (1,) int32, index of free_pages to take pages from (None:
+            0); what a call returns goes into the next one.
         validate: check the lengths and the room in the packed rows and
             the block table (see the module's documentation).  With False,
             negative lengths count as 0.
@@ -128,7 +128,10 @@ def paged_kvcache_slots(block_table, cache_seqlens, new_seqlens, free_pages, pag
     Pages go to the requests in order.  Where the free ones do not reach, a
     request that needs any gets none: its slots are -1 (an append skips them),
     its length and its row of the table stay as they were.  That is no error:
-    a scheduler compares the returned lengths with the ones it asked for.
+    a scheduler compares the returned lengths with the ones it asked for, and
+    comes with a new list.  Until then nobody overtakes a refused request: the
+    returned index counts the pages needed up to the last request served,
+    with those of refused requests in between, and may lie past the list.
     """
     if not isinstance(block_table, torch.Tensor) or block_table.ndim != 2 or block_table.dtype != torch.int32:
         raise ValueError("block_table must be an int32 tensor of shape (batch, max_num_pages)")
@@ -162,8 +165,7 @@ def paged_kvcache_slots(block_table, cache_seqlens, new_seqlens, free_pages, pag
             if batch:
                 total = chk.value(new_seqlens.sum())
             if free_start is not None:
-                chk.check_range(free_start, 0, free_pages.shape[0],
-                                ValueError("free_start must index free_pages"))
+                chk.check_range(free_start, 0, None, ValueError("free_start must be non-negative"))
             values = chk.flush()
             if batch and values[total] > max_tokens:
                 raise ValueError("max_tokens must cover the new tokens of every request")

@@ -436,11 +436,14 @@ int fa_check_wait(const int64_t* result, int n, fa_stream_t stream);
  * sequence) and slot_mapping (page * page_size + position % page_size).
  * max_tokens is the number of packed rows; rows past the last request get slot
  * -1 and position 0.  cu_seqlens [batch + 1] are the prefix sums of
- * new_seqlens (at most max_tokens), seqlens_out the lengths afterwards and
- * free_end[0] the index of the first free page left.  A request is refused
- * (slots -1, its length and table row as they were) if it passes the end of
- * its table row or of the packed rows, or if it needs pages and those needed
- * up to and with it are more than are free.  Lengths below 0 count as 0.
+ * new_seqlens (at most max_tokens), seqlens_out the lengths afterwards.  A
+ * request is refused (slots -1, its length and table row as they were) if it
+ * passes the end of its table row or of the packed rows, or if it needs pages
+ * and those needed up to and with it are more than are free.  free_end[0] is
+ * the index to go on from: free_start plus the pages needed up to and with the
+ * last request served, refused ones in between (of those that fit their row)
+ * included, so that requests behind a refused one do not overtake it in later
+ * calls either; it may then lie past the list.  Lengths below 0 count as 0.
  * Nothing is read or written outside the arrays whatever they hold. */
 int fa_kvcache_slots(int32_t* block_table, int64_t block_table_stride, int64_t cols,
                      const int32_t* cache_seqlens, const int32_t* new_seqlens, int64_t batch,

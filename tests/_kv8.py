@@ -153,16 +153,16 @@ def attend(q, kc, ks, vc, vs, lens, table, cu=None, scale=None, causal=False, wi
 def slots_of(table, cached, added, free, page, rows, start=0):
     """paged_kvcache_slots in Python: (table, slots, positions, cu, seqlens, free_start)."""
     table = [list(t) for t in table]
-    slots, pos, cu, lens, row, at, wanted = [-1] * rows, [0] * rows, [0], [], 0, start, start
+    slots, pos, cu, lens, row, end, wanted = [-1] * rows, [0] * rows, [0], [], 0, start, start
     for b, (o, n) in enumerate(zip(cached, added)):
         have, upto = -(-o // page), -(-(o + n) // page)
         ok = upto <= len(table[b]) and row + n <= rows
-        if ok and upto > have:
+        if ok:
             wanted += upto - have
-            ok = wanted <= len(free)
-            if ok:
-                table[b][have:upto] = free[at:wanted]
-                at = wanted
+            ok = upto == have or wanted <= len(free)
+        if ok:
+            table[b][have:upto] = free[wanted - (upto - have):wanted] if upto > have else []
+            end = wanted
         for i in range(n):
             if row + i < rows:
                 pos[row + i] = o + i
@@ -171,4 +171,4 @@ def slots_of(table, cached, added, free, page, rows, start=0):
         row += n
         cu.append(min(row, rows))
         lens.append(o + n if ok else o)
-    return table, slots, pos, cu, lens, at
+    return table, slots, pos, cu, lens, end

@@ -79,6 +79,16 @@ def test_slots_with_too_few_pages(batch):
         _check_slots(table, cached, added, free[:left] or [0][:left], 16, rows)
     _check_slots(table, cached, added, free, 16, rows, start=3)
     _check_slots(table, cached, added, free, 16, rows, start=len(free))
+    _check_slots(table, cached, added, free, 16, rows, start=len(free) + 9)
+
+
+def test_slots_refused_requests_are_not_overtaken():
+    # request 1 needs 3 of 2 pages, request 2 none, request 3 one: the index passes the list, and stays there
+    table = [[0, -1, -1, -1], [1, -1, -1, -1], [2, -1, -1, -1], [3, -1, -1, -1]]
+    cached, added, free = [16, 16, 5, 16], [1, 48, 1, 0], [7, 8, 9]
+    _check_slots(table, cached, added, free, 16, 60)
+    t, got = _run_slots(table, cached, added, free, 16, 60)
+    assert got[3].tolist() == [17, 16, 6, 16] and got[4].tolist() == [4]
 
 
 def test_slots_without_tokens_or_requests():
@@ -115,8 +125,8 @@ def test_slots_refusals():
         _run_slots([[0, 1]], [20], [13], [5], 16, 40)
     with pytest.raises(ValueError, match="max_tokens must cover"):
         _run_slots([[0, 1]], [20], [5], [5], 16, 4)
-    with pytest.raises(ValueError, match="free_start must index"):
-        _run_slots([[0, 1]], [20], [5], [5], 16, 5, start=2)
+    with pytest.raises(ValueError, match="free_start must be"):
+        _run_slots([[0, 1]], [20], [5], [5], 16, 5, start=-1)
 
 
 # ----------------------------------------------------------------------------- append
