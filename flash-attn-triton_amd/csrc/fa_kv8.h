@@ -59,9 +59,17 @@ struct Kv8AttnParams {
   float scale, softcap;
   const float* alibi; int64_t alibi_sb;
   int causal, window_left, window_right;
-  int row_blocks, split_keys, num_splits;
+  // Sequences of at most 32 rows (queries times the group) per K/V head:
+  // kv8_split_kernel, their keys in num_splits splits of split_keys (0: there are
+  // none).  The others: kv8_chunk_kernel, chunk_blocks blocks of chunk_rows rows.
+  int split_keys, num_splits;
+  int chunk_rows, chunk_blocks, chunk_keys, chunk_splits;
   float* o_part; float* lse_part;   // [split][row of q][head](D); LSE in log2 units
 };
+
+constexpr int kKv8SplitRows = 32;
+constexpr int kKv8ChunkRows = 128;
+constexpr int kKv8MaxSplit = 4096;   // keys whose pages the lanes of a workgroup's waves hold
 
 }  // namespace fa
 

@@ -68,27 +68,41 @@ int check_cache(const char* name, int64_t num_pages, int64_t page_size, int64_t 
 }
 
 struct Plan {
-  int row_blocks, split_keys, num_splits;
+  int split_keys, num_splits, chunk_blocks, chunk_keys, chunk_splits;
   int64_t workspace;
 };
 
-// Keys per split: the largest of 4096 .. 256 that leaves every CU several
-// workgroups, else 128 (a tile per wave).
-Plan make_plan(int64_t batch, int64_t seqlen_q, int64_t total_q, int64_t heads_q, int64_t heads_k,
-               int64_t head_dim, int64_t max_keys) {
-  Plan pl;
-  const int64_t group = heads_q / heads_k;
-  pl.row_blocks = (int)((seqlen_q * group + 31) / 32);
-  const int64_t items = batch * heads_k * pl.row_blocks;
-  pl.split_keys = 128;
-  for (int sk = 4096; sk >= 256; sk /= 2)
-    if (items * ((max_keys + sk - 1) / sk) >= 2048) {
-      pl.split_keys = sk;
-      break;
-    }
-  const int64_t n = (max_keys + pl.split_keys - 1) / pl.split_keys;
-  pl.num_splits = (int)(n < 1 ? 1 : n);
-  pl.workspace = pl.num_splits > 1 ? pl.num_splits * total_q * heads_q * (head_dim + 1) * 4 : 0;
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// How the keys are split.  Packed queries may hold sequences for both kernels;
+// the host only knows the longest.
+Plan make_plan(bool packed, int64_t batch, int64_t seqlen_q, int64_t total_q, int64_t heads_q,
+               int64_t heads_k, int64_t head_dim, int64_t max_keys) {
+  Plan pl = {};
+  const int64_t group = heads_q / heads_k, rows = seqlen_q * group;
+  if (packed || rows <= fa::kKv8SplitRows) {
+    // The largest of 4096 .. 256 keys that leaves every CU several workgroups,
+    // else 128 (a tile per wave).
+    pl.split_keys = 128;
+    for (int sk = fa::kKv8MaxSplit; sk >= 256; sk /= 2)
+      if (batch * heads_k * ceil_div(max_keys, sk) >= 2048) {
+        pl.split_keys = sk;
+        break;
+      }
+    pl.num_splits = (int)ceil_div(max_keys > 0 ? max_keys : 1, pl.split_keys);
+  }
+  if (rows > fa::kKv8SplitRows) {
+    pl.chunk_blocks = (int)ceil_div(rows, fa::kKv8ChunkRows);
+    const int64_t most = batch * pl.chunk_blocks, by_rows = ceil_div(total_q * group, fa::kKv8ChunkRows) + batch;
+    const int64_t wgs = heads_k * (most < by_rows ? most : by_rows);
+    int64_t n = wgs >= 256 ? 1 : ceil_div(512, wgs);
+    const int64_t cap = ceil_div(max_keys > 0 ? max_keys : 1, 512);
+    n = n < cap ? n : cap;
+    pl.chunk_keys = (int)(ceil_div(ceil_div(max_keys > 0 ? max_keys : 1, n), 64) * 64);
+    pl.chunk_splits = (int)ceil_div(max_keys > 0 ? max_keys : 1, pl.chunk_keys);
+  }
+  const int most = pl.num_splits > pl.chunk_splits ? pl.num_splits : pl.chunk_splits;
+  pl.workspace = most > 1 ? most * total_q * heads_q * (head_dim + 1) * 4 : 0;
   return pl;
 }
 
@@ -200,16 +214,15 @@ extern "C" int fa_kvcache8_append(const void* k, const void* v, const int64_t* k
   return hip_status(fa_launch_kv8_append(dtype, store, p, (int)head_dim, static_cast<hipStream_t>(stream)), name);
 }
 
-extern "C" int fa_fwd_kvcache8_plan(int64_t batch, int64_t max_seqlen_q, int64_t total_q, int64_t heads_q,
-                                    int64_t heads_k, int64_t head_dim, int64_t max_keys, int32_t* num_splits,
+extern "C" int fa_fwd_kvcache8_plan(int packed, int64_t batch, int64_t max_seqlen_q, int64_t total_q,
+                                    int64_t heads_q, int64_t heads_k, int64_t head_dim, int64_t max_keys,
                                     int64_t* workspace_bytes) {
   const char* name = "fa_fwd_kvcache8_plan";
-  if (num_splits == nullptr || workspace_bytes == nullptr) return fail(FA_ERR_INVALID, "%s: null pointer", name);
+  if (workspace_bytes == nullptr) return fail(FA_ERR_INVALID, "%s: null pointer", name);
   if (int st = check_plan(name, batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys); st != FA_OK)
     return st;
-  const Plan pl = make_plan(batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys);
-  *num_splits = pl.num_splits;
-  *workspace_bytes = pl.workspace;
+  *workspace_bytes =
+      make_plan(packed != 0, batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys).workspace;
   return fa_set_error(FA_OK, "");
 }
 
@@ -223,8 +236,8 @@ extern "C" int fa_fwd_kvcache8(const void* q, void* out, const int64_t* q_stride
                                int64_t max_seqlen_q, int64_t total_q, int64_t max_keys, int64_t heads_q,
                                int64_t heads_k, int64_t head_dim, float softmax_scale, int causal,
                                int64_t window_left, int64_t window_right, float softcap,
-                               const float* alibi_slopes, int64_t alibi_batch_stride, int32_t num_splits,
-                               void* workspace, int64_t workspace_bytes, fa_stream_t stream) {
+                               const float* alibi_slopes, int64_t alibi_batch_stride, void* workspace,
+                               int64_t workspace_bytes, fa_stream_t stream) {
   const char* name = "fa_fwd_kvcache8";
   if (int st = check_plan(name, batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys); st != FA_OK)
     return st;
@@ -251,9 +264,10 @@ extern "C" int fa_fwd_kvcache8(const void* q, void* out, const int64_t* q_stride
   if (k_cache_stride[1] < head_dim || v_cache_stride[1] < head_dim || k_cache_stride[1] > kMaxSlotStride ||
       v_cache_stride[1] > kMaxSlotStride)
     return fail(FA_ERR_UNSUPPORTED, "%s: slots that overlap or lie more than 2^26 bytes apart", name);
-  const Plan pl = make_plan(batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys);
-  if (num_splits != pl.num_splits || workspace_bytes < pl.workspace || (pl.workspace > 0 && workspace == nullptr))
-    return fail(FA_ERR_INVALID, "%s: num_splits and workspace must come from fa_fwd_kvcache8_plan", name);
+  const Plan pl =
+      make_plan(cu_seqlens_q != nullptr, batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys);
+  if (workspace_bytes < pl.workspace || (pl.workspace > 0 && workspace == nullptr))
+    return fail(FA_ERR_INVALID, "%s: the workspace must be as large as fa_fwd_kvcache8_plan says", name);
   fa::Kv8AttnParams p;
   p.q = q;
   p.o = out;
@@ -288,11 +302,14 @@ extern "C" int fa_fwd_kvcache8(const void* q, void* out, const int64_t* q_stride
   p.causal = causal != 0;
   p.window_left = clamp_window(window_left);
   p.window_right = clamp_window(window_right);
-  p.row_blocks = pl.row_blocks;
   p.split_keys = pl.split_keys;
   p.num_splits = pl.num_splits;
+  p.chunk_rows = fa::kKv8ChunkRows;
+  p.chunk_blocks = pl.chunk_blocks;
+  p.chunk_keys = pl.chunk_keys;
+  p.chunk_splits = pl.chunk_splits;
   p.o_part = static_cast<float*>(workspace);
-  p.lse_part = pl.workspace > 0 ? p.o_part + (int64_t)pl.num_splits * total_q * heads_q * head_dim : nullptr;
+  p.lse_part = p.o_part + pl.workspace / 4 / (head_dim + 1) * head_dim;
   hipStream_t st = static_cast<hipStream_t>(stream);
   return hip_status(dtype == FA_DTYPE_F16 ? fa_launch_kv8_attn_f16(store, p, (int)head_dim, st)
                                           : fa_launch_kv8_attn_bf16(store, p, (int)head_dim, st),

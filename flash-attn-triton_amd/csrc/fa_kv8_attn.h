@@ -38,7 +38,7 @@ namespace fa {
 
 constexpr int kKv8Waves = 4;
 constexpr int kKv8BN = 32;            // keys of a tile
-constexpr int kKv8MaxSplit = 32 * kKv8Waves * kKv8BN;   // 64 lanes hold the groups of 32 tiles per wave
+static_assert(kKv8MaxSplit == 32 * kKv8Waves * kKv8BN, "64 lanes hold the 16-key groups of 32 tiles");
 
 // The 8-bit types.  bad(): the high bit of each byte of a word whose number is
 // not finite.
@@ -149,6 +149,145 @@ __device__ inline void kv8_key_range(const Kv8AttnParams& p, const Kv8Rows& s, i
   hi = max(hi, 0);
 }
 
+// What a query row of a lane sees and how its scores are scaled.
+struct Kv8Row {
+  int key_lo, key_hi, qpos;
+  float slope;
+};
+
+template <bool GENERIC>
+__device__ inline Kv8Row kv8_row(const Kv8AttnParams& p, const Kv8Rows& s, int qi, int head, int k_end) {
+  Kv8Row r;
+  r.qpos = qi + (p.causal ? s.L - s.n : 0);
+  r.key_lo = 0;
+  r.key_hi = k_end - 1;   // (the workgroup's keys end there)
+  if (p.causal) r.key_hi = min(r.key_hi, r.qpos);
+  if (p.window_right >= 0) r.key_hi = min(r.key_hi, r.qpos + p.window_right);
+  if (p.window_left >= 0) r.key_lo = max(0, r.qpos - p.window_left);
+  r.slope = GENERIC && p.alibi != nullptr ? p.alibi[(int64_t)s.b * p.alibi_sb + head] : 0.f;
+  return r;
+}
+
+// S^T of 32 keys: LDS rows row0 .. row0 + 31 of a K tile against Q^T in
+// registers, the rows scaled by ksc (one value per lane: its key's).
+template <class T, class F8, int D>
+__device__ inline f32x16 kv8_qk(const uint8_t* kt, int row0, float ksc, const u32x4* qreg) {
+  const int lane = threadIdx.x & 63, row = row0 + (lane & 31), g = lane >> 5;
+  f32x16 sc = f32x16{};
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+    const u32x4 raw = load16(kt + row * D + kv8_k_chunk<D>(row, 2 * j + g) * 16);
+    sc = T::mfma32(kv8_operand<T, F8>(raw[0], raw[1], ksc), qreg[2 * j], sc);
+    sc = T::mfma32(kv8_operand<T, F8>(raw[2], raw[3], ksc), qreg[2 * j + 1], sc);
+  }
+  return sc;
+}
+
+// Scale, ALiBi and softcap of the scores of keys n0 .. n0 + 31.
+__device__ inline void kv8_score_options(const Kv8AttnParams& p, const Kv8Row& row, int n0, f32x16& sc) {
+  const int g = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    const int key = n0 + 8 * (v >> 2) + 4 * g + (v & 3);
+    float x = sc[v] * p.scale;
+    x = fmaf(-row.slope, fabsf((float)(row.qpos - key)), x);
+    if (p.softcap > 0.f) {
+      // softcap tanh(x / softcap) = softcap (1 - 2 / (exp(2 x / softcap) + 1))
+      const float ex = __builtin_amdgcn_exp2f(x * (2.f * kLog2e / p.softcap));
+      x = p.softcap * (1.f - 2.f / (ex + 1.f));
+    }
+    sc[v] = x;
+  }
+}
+
+__device__ inline void kv8_mask(const Kv8Row& row, int n0, f32x16& sc) {
+  const int g = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    const int key = n0 + 8 * (v >> 2) + 4 * g + (v & 3);
+    if (key < row.key_lo || key > row.key_hi) sc[v] = -INFINITY;
+  }
+}
+
+// P of 32 keys, packed to 16 bits as the B operand of two 16-key steps, its
+// fp32 sum added to l.
+template <class T>
+__device__ inline void kv8_exp(const f32x16& sc, float sl, float m, u32x4* pb, float& l) {
+#pragma unroll
+  for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[cc * 8 + 2 * j], sl, -m));
+      const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[cc * 8 + 2 * j + 1], sl, -m));
+      pb[cc][j] = T::pack2(e0, e1);
+      l += e0 + e1;
+    }
+}
+
+// O^T += V^T P^T over the 32 keys of LDS rows row0 .. of a V tile, scaled by
+// vsc (16 keys each).  mixed: the rows of the wave do not all see all of these
+// keys, and a V number that is not finite must not meet a P of 0.
+template <class T, class F8, int D>
+__device__ inline void kv8_pv(const uint8_t* vt, int row0, const float* vsc, const u32x4* pb,
+                              const f32x16& sc, bool mixed, f32x16* acc) {
+  constexpr int NDB = D / 32;
+  const int lane = threadIdx.x & 63, g = lane >> 5;
+  // The lane's 8 keys of step cc are 16 cc + 4 g + {0..3, 8..11}: row i / 2 of
+  // the transposed read, i the lane among its 16.
+  const int vr = (lane & 15) >> 1, vkey = 4 * g + (vr & 3) + 8 * (vr >> 2);
+  const int vc = (lane >> 4) & 1, vh = 8 * (lane & 1);
+  u32x2 raw[2][NDB];
+#pragma unroll
+  for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      const int row = row0 + 16 * cc + vkey;
+      raw[cc][db] = lds_read_tr8(vt + row * D + kv8_v_chunk<D>(row, 2 * db + vc) * 16 + vh);
+    }
+  if (mixed) {
+    uint32_t flags = 0;
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) flags |= F8::bad(raw[cc][db][0]) | F8::bad(raw[cc][db][1]);
+    if (__builtin_amdgcn_ballot_w64(flags != 0) != 0) {
+      // Visible (key, row) pairs and numbers that are not finite, as 1 and 0: a
+      // row gets NaN in the columns where their product is not zero.
+      u32x4 seen[2];
+#pragma unroll
+      for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          seen[cc][j] = T::pack2(sc[cc * 8 + 2 * j] == -INFINITY ? 0.f : 1.f,
+                                 sc[cc * 8 + 2 * j + 1] == -INFINITY ? 0.f : 1.f);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        f32x16 hit = f32x16{};
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          u32x4 ind;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t f = F8::bad(raw[cc][db][e]);
+            ind[2 * e] = T::pack2((f & 0x80u) ? 1.f : 0.f, (f & 0x8000u) ? 1.f : 0.f);
+            ind[2 * e + 1] = T::pack2((f & 0x800000u) ? 1.f : 0.f, (f & 0x80000000u) ? 1.f : 0.f);
+            raw[cc][db][e] &= ~((f >> 7) * 0xffu);
+          }
+          hit = T::mfma32(ind, seen[cc], hit);
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (hit[v] > 0.f) acc[db][v] = __uint_as_float(0x7fc00000u);
+      }
+    }
+  }
+#pragma unroll
+  for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+      acc[db] = T::mfma32(kv8_operand<T, F8>(raw[cc][db][0], raw[cc][db][1], vsc[cc]), pb[cc], acc[db]);
+}
+
 template <int D, int NST>
 struct Kv8Tile {
   static constexpr int kBytes = kKv8BN * D;            // one tile of K or V
@@ -181,43 +320,33 @@ void kv8_split_kernel(const Kv8AttnParams p) {
   int id = blockIdx.x;
   const int kvh = id % p.heads_k;
   id /= p.heads_k;
-  const int rb = id % p.row_blocks;
-  id /= p.row_blocks;
   const int b = id % p.batch;
   const int split = id / p.batch;
 
   const Kv8Rows s = kv8_rows(p, b);
   const int G = (int)p.group.d;
-  const int rows = min(s.n * G - rb * 32, 32);
-  if (rows <= 0) return;
-  const int q_first = (int)fdiv(rb * 32, p.group), q_last = (int)fdiv(rb * 32 + rows - 1, p.group);
+  const int rows = s.n * G;
+  if (rows <= 0 || rows > kKv8SplitRows) return;
   int lo, hi;
-  kv8_key_range(p, s, q_first, q_last, lo, hi);
+  kv8_key_range(p, s, 0, s.n - 1, lo, hi);
   // This split's keys.  Split 0 always runs, so that rows without keys are
   // written when there is no combine.
   const int k_begin = max(split * p.split_keys, lo & ~(BN - 1));
   const int k_end = min(hi, (split + 1) * p.split_keys);
   if (k_begin >= k_end && split > 0) return;
 
-  const int r = min(c32, rows - 1);
+  const int r = min(c32, rows - 1);   // (lanes past the last row repeat it)
   const bool row_valid = c32 < rows;
-  const int qi = (int)fdiv(rb * 32 + r, p.group);
-  const int head = kvh * G + (rb * 32 + r - qi * G);
+  const int qi = (int)fdiv(r, p.group);
+  const int head = kvh * G + (r - qi * G);
   const int off = p.causal ? s.L - s.n : 0;
-  const int qpos = qi + off;
-  int key_hi = s.L - 1, key_lo = 0;
-  if (p.causal) key_hi = min(key_hi, qpos);
-  if (p.window_right >= 0) key_hi = min(key_hi, qpos + p.window_right);
-  if (p.window_left >= 0) key_lo = max(0, qpos - p.window_left);
+  Kv8Row row = kv8_row<GENERIC>(p, s, qi, head, k_end);
   // Keys that every row sees: tiles within need no mask.
   int all_lo = 0, all_hi = s.L - 1;
-  if (p.causal) all_hi = min(all_hi, q_first + off);
-  if (p.window_right >= 0) all_hi = min(all_hi, q_first + off + p.window_right);
-  if (p.window_left >= 0) all_lo = max(0, q_last + off - p.window_left);
-  float slope = 0.f;
-  if (GENERIC && p.alibi != nullptr) slope = p.alibi[(int64_t)b * p.alibi_sb + head];
-
-  // Q^T in the order of the K operand (rows past the last repeat it).
+  if (p.causal) all_hi = min(all_hi, off);
+  if (p.window_right >= 0) all_hi = min(all_hi, off + p.window_right);
+  if (p.window_left >= 0) all_lo = max(0, s.n - 1 + off - p.window_left);
+  // Q^T in the order of the K operand.
   u32x4 qreg[2 * NDB];
   {
     const uint16_t* qrow = static_cast<const uint16_t*>(p.q) + kv8_base(p, s, p.q_sb, p.q_ss) +
@@ -297,7 +426,8 @@ void kv8_split_kernel(const Kv8AttnParams p) {
   // are waited for here, once.
 #pragma unroll
   for (int j = 0; j < 2 * NDB; ++j) asm volatile("" : "+v"(qreg[j]));
-  asm volatile("" : "+v"(ks_l), "+v"(vs_l), "+v"(slope));
+  asm volatile("" : "+v"(ks_l), "+v"(vs_l));
+  if (GENERIC) asm volatile("" : "+v"(row.slope));
   for (int t = 0; t < my_tiles; ++t) {
     const int n0 = k_begin + (w + t * kKv8Waves) * BN;
     // (this wave's LDS reads of the stage that is filled now ended with the
@@ -311,38 +441,10 @@ void kv8_split_kernel(const Kv8AttnParams p) {
 
     const float ks0 = __uint_as_float(__builtin_amdgcn_readlane(ks_l, 2 * t));
     const float ks1 = __uint_as_float(__builtin_amdgcn_readlane(ks_l, 2 * t + 1));
-    const float ksc = c32 < 16 ? ks0 : ks1;
-    f32x16 sc = f32x16{};
-#pragma unroll
-    for (int j = 0; j < NDB; ++j) {
-      const u32x4 raw = load16(kt + c32 * D + kv8_k_chunk<D>(c32, 2 * j + g) * 16);
-      sc = T::mfma32(kv8_operand<T, F8>(raw[0], raw[1], ksc), qreg[2 * j], sc);
-      sc = T::mfma32(kv8_operand<T, F8>(raw[2], raw[3], ksc), qreg[2 * j + 1], sc);
-    }
-
-    const bool masked = n0 < all_lo || n0 + BN - 1 > all_hi;
+    f32x16 sc = kv8_qk<T, F8, D>(kt, 0, c32 < 16 ? ks0 : ks1, qreg);
+    if (GENERIC) kv8_score_options(p, row, n0, sc);
+    if (n0 < all_lo || n0 + BN - 1 > all_hi) kv8_mask(row, n0, sc);
     float mx = -INFINITY;
-    if (GENERIC) {
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int key = n0 + 8 * (v >> 2) + 4 * g + (v & 3);
-        float x = sc[v] * p.scale;
-        if (p.alibi != nullptr) x = fmaf(-slope, fabsf((float)(qpos - key)), x);
-        if (p.softcap > 0.f) {
-          // softcap * tanh(x / softcap) = softcap * (1 - 2 / (exp(2 x / softcap) + 1))
-          const float ex = __builtin_amdgcn_exp2f(x * (2.f * kLog2e / p.softcap));
-          x = p.softcap * (1.f - 2.f / (ex + 1.f));
-        }
-        sc[v] = x;
-      }
-    }
-    if (masked) {
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int key = n0 + 8 * (v >> 2) + 4 * g + (v & 3);
-        if (key < key_lo || key > key_hi || key >= k_end) sc[v] = -INFINITY;
-      }
-    }
 #pragma unroll
     for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[v]);
     mx = halves_max(mx) * sl;
@@ -354,78 +456,16 @@ void kv8_split_kernel(const Kv8AttnParams p) {
       for (int db = 0; db < NDB; ++db) acc[db] *= alpha;
       m_run = m_new;
     }
-    const float m_use = m_run == -INFINITY ? 0.f : m_run;
     u32x4 pb[2];
-#pragma unroll
-    for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[cc * 8 + 2 * j], sl, -m_use));
-        const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[cc * 8 + 2 * j + 1], sl, -m_use));
-        pb[cc][j] = T::pack2(e0, e1);
-        l_run += e0 + e1;
-      }
+    kv8_exp<T>(sc, sl, m_run == -INFINITY ? 0.f : m_run, pb, l_run);
 
     __builtin_amdgcn_s_waitcnt(vmcnt_imm((NST - 1) * 2 * NI));   // V of tile t
     asm volatile("" ::: "memory");
-    // The lane's 8 keys of step cc: 16 cc + 4 g + {0..3, 8..11}; row i / 2 of
-    // the transposed read, i the lane among its 16.
-    const int vr = (lane & 15) >> 1, vkey = 4 * g + (vr & 3) + 8 * (vr >> 2);
-    const int vc = ((lane >> 4) & 1), vh = 8 * (lane & 1);
-    uint32_t flags = 0;
-    u32x2 raw[2][NDB];
-#pragma unroll
-    for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        const int row = 16 * cc + vkey;
-        raw[cc][db] = lds_read_tr8(vt + row * D + kv8_v_chunk<D>(row, 2 * db + vc) * 16 + vh);
-      }
+    const float vsc[2] = {__uint_as_float(__builtin_amdgcn_readlane(vs_l, 2 * t)),
+                          __uint_as_float(__builtin_amdgcn_readlane(vs_l, 2 * t + 1))};
+    // (keys past the sequence's end are zeros in V)
     const bool mixed = n0 < all_lo || (n0 + BN - 1 > all_hi && all_hi < s.L - 1);
-    if (mixed) {
-#pragma unroll
-      for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) flags |= F8::bad(raw[cc][db][0]) | F8::bad(raw[cc][db][1]);
-    }
-    const bool dirty = mixed && __builtin_amdgcn_ballot_w64(flags != 0) != 0;
-    if (dirty) {
-      // Visible (key, row) pairs and numbers that are not finite, as 1 and 0: a
-      // row gets NaN in the columns where their product is not zero.
-      u32x4 seen[2];
-#pragma unroll
-      for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          seen[cc][j] = T::pack2(sc[cc * 8 + 2 * j] == -INFINITY ? 0.f : 1.f,
-                                 sc[cc * 8 + 2 * j + 1] == -INFINITY ? 0.f : 1.f);
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        f32x16 hit = f32x16{};
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          u32x4 ind;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t f = F8::bad(raw[cc][db][e]);
-            ind[2 * e] = T::pack2((f & 0x80u) ? 1.f : 0.f, (f & 0x8000u) ? 1.f : 0.f);
-            ind[2 * e + 1] = T::pack2((f & 0x800000u) ? 1.f : 0.f, (f & 0x80000000u) ? 1.f : 0.f);
-            raw[cc][db][e] &= ~((f >> 7) * 0xffu);
-          }
-          hit = T::mfma32(ind, seen[cc], hit);
-        }
-#pragma unroll
-        for (int v = 0; v < 16; ++v)
-          if (hit[v] > 0.f) acc[db][v] = __uint_as_float(0x7fc00000u);
-      }
-    }
-#pragma unroll
-    for (int cc = 0; cc < 2; ++cc) {
-      const float vsc = __uint_as_float(__builtin_amdgcn_readlane(vs_l, 2 * t + cc));
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-        acc[db] = T::mfma32(kv8_operand<T, F8>(raw[cc][db][0], raw[cc][db][1], vsc), pb[cc], acc[db]);
-    }
+    kv8_pv<T, F8, D>(vt, 0, vsc, pb, sc, mixed, acc);
   }
 
   // ------------------------------------------------------------ merge waves
@@ -481,8 +521,8 @@ void kv8_split_kernel(const Kv8AttnParams p) {
       for (int k = 0; k < 4; ++k) o[e + k] = fmaf(x[k], wt[u], o[e + k]);
     }
   }
-  const int oi = (int)fdiv(rb * 32 + rr, p.group);
-  const int oh = kvh * G + (rb * 32 + rr - oi * G);
+  const int oi = (int)fdiv(rr, p.group);
+  const int oh = kvh * G + (rr - oi * G);
   if (p.num_splits == 1) {
     uint16_t* dst = static_cast<uint16_t*>(p.o) + kv8_base(p, s, p.o_sb, p.o_ss) +
                     (int64_t)oi * p.o_ss + (int64_t)oh * p.o_sh + d0;
@@ -504,6 +544,310 @@ void kv8_split_kernel(const Kv8AttnParams p) {
   }
 }
 
+
+// kv8_chunk_kernel: more than 32 query rows per K/V head.  A workgroup of RW x
+// KG waves owns 32 RW rows, 32 per wave; its KG groups of RW waves take the
+// 64-key tiles in turn (each group with a ring of its own, whose tiles its waves
+// load together) and are merged at the end, so that a workgroup's chain of
+// tiles is KG times shorter: rows of long sequences beside those of short ones
+// would otherwise set the launch's time.  Tile operands, masks and scales as in
+// kv8_split_kernel; pages and scales of up to NT 16-key groups are in LDS at a time
+// (NT threads).
+template <int D, int RW, int KG, int NST>
+struct Kv8Chunk {
+  static constexpr int kBN = 64;
+  static constexpr int kThreads = RW * KG * 64;
+  static constexpr int kTile = kBN * D;                     // bytes of a K or V tile
+  static constexpr int kRings = KG * NST * 2 * kTile;
+  static constexpr int kWave = 32 * (D + 2) * 4;            // a wave's rows, maxima and sums in fp32
+  static constexpr int kMerge = (KG > 1 ? KG - 1 : 1) * RW * kWave;
+  static constexpr int kInfo = kThreads * 12;
+  static constexpr int kLds = (kRings > kMerge ? kRings : kMerge) + kInfo;
+  static constexpr int kSuper = kThreads * 16 / kBN;        // tiles whose pages and scales LDS holds
+};
+
+// The r-th sequence by descending work (queries times keys; r counted within
+// its block of 64 consecutive ones): long ones first, so that they do not start
+// last.  Every lane of the wave takes part.
+__device__ inline int kv8_nth_heaviest(const Kv8AttnParams& p, int r) {
+  const int base = r & ~63, m = min(64, p.batch - base), l = threadIdx.x & 63;
+  uint32_t key = 0;
+  if (l < m) {
+    const Kv8Rows s = kv8_rows(p, base + l);
+    // (unique: the work in 25 bits of its order of magnitude, then the earlier one)
+    const float work = (float)s.n * (float)s.L;
+    key = ((__float_as_uint(work) >> 6) & ~63u) + 64u + (uint32_t)(63 - l);
+  }
+  int rank = 0;
+  for (int j = 0; j < m; ++j) rank += (uint32_t)__builtin_amdgcn_readlane(key, j) > key ? 1 : 0;
+  const uint64_t hit = __builtin_amdgcn_ballot_w64(l < m && rank == (r & 63));
+  return base + (hit != 0 ? (int)__builtin_ctzll(hit) : 0);
+}
+
+template <class T, class F8, int D, int RW, int KG, int NST, bool GENERIC>
+__global__ __launch_bounds__(RW * KG * 64) __attribute__((amdgpu_waves_per_eu(RW * KG / 4)))
+void kv8_chunk_kernel(const Kv8AttnParams p) {
+  using C = Kv8Chunk<D, RW, KG, NST>;
+  constexpr int BN = C::kBN, BM = 32 * RW;
+  constexpr int CPR = D / 16, RPI = 64 / CPR, IPG = 16 / RPI, NDB = D / 32;
+  constexpr int GPW = 4 / RW;                  // 16-key groups of a tile that a wave loads
+  constexpr int PER = 2 * GPW * IPG;           // its DMA instructions per tile
+  static_assert(RW == 2 || RW == 4, "a wave loads whole 16-key groups");
+
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem8c[];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rw = w % RW, kg = w / RW;
+  const int c32 = lane & 31, g = lane >> 5;
+
+  // Work item: the K/V heads of the sequences, heaviest sequence first, are
+  // dealt round over the XCDs, all row blocks (and splits) of one on the same, so
+  // that they share its keys in the L2; the last ones, too few for a round, are
+  // spread over all.
+  const int per = p.chunk_blocks * p.chunk_splits;
+  const int main = p.batch * p.heads_k / 8 * 8;
+  int item = blockIdx.x, c, i;
+  if (item < main * per) {
+    const int k = item / 8;
+    c = k / per * 8 + item % 8;
+    i = k % per;
+  } else {
+    item -= main * per;
+    c = main + item / per;
+    i = item % per;
+  }
+  const int b = kv8_nth_heaviest(p, c / p.heads_k);
+  const int kvh = c % p.heads_k;
+  const int rb = p.chunk_blocks - 1 - i / p.chunk_splits, split = i % p.chunk_splits;
+
+  const Kv8Rows s = kv8_rows(p, b);
+  const int G = (int)p.group.d;
+  const int rows = min(s.n * G - rb * BM, BM);
+  if (rows <= 0 || s.n * G <= kKv8SplitRows) return;
+  int lo, hi;
+  kv8_key_range(p, s, (int)fdiv(rb * BM, p.group), (int)fdiv(rb * BM + rows - 1, p.group), lo, hi);
+  const int k_begin = max(split * p.chunk_keys, lo & ~(BN - 1));
+  const int k_end = min(hi, (split + 1) * p.chunk_keys);
+  if (k_begin >= k_end && split > 0) return;
+
+  // This wave's rows (it helps to load when it has none) and the keys that all
+  // of them see.
+  const int r0 = rb * BM + rw * 32;
+  const int wrows = max(min(rows - rw * 32, 32), 0);
+  const bool row_valid = c32 < wrows;
+  const int r = r0 + max(min(c32, wrows - 1), 0) - (wrows > 0 ? 0 : rw * 32);
+  const int qi = (int)fdiv(r, p.group);
+  const int head = kvh * G + (r - qi * G);
+  const int q_first = (int)fdiv(wrows > 0 ? r0 : rb * BM, p.group);
+  const int q_last = wrows > 0 ? (int)fdiv(r0 + wrows - 1, p.group) : q_first;
+  const int off = p.causal ? s.L - s.n : 0;
+  Kv8Row row = kv8_row<GENERIC>(p, s, qi, head, k_end);
+  int all_lo = 0, all_hi = s.L - 1;
+  if (p.causal) all_hi = min(all_hi, q_first + off);
+  if (p.window_right >= 0) all_hi = min(all_hi, q_first + off + p.window_right);
+  if (p.window_left >= 0) all_lo = max(0, q_last + off - p.window_left);
+  int wlo, whi;   // keys that any of the wave's rows sees
+  kv8_key_range(p, s, q_first, q_last, wlo, whi);
+  if (wrows == 0) whi = 0;
+
+  u32x4 qreg[2 * NDB];
+  {
+    const uint16_t* qrow = static_cast<const uint16_t*>(p.q) + kv8_base(p, s, p.q_sb, p.q_ss) +
+                           (int64_t)qi * p.q_ss + (int64_t)head * p.q_sh;
+#pragma unroll
+    for (int j = 0; j < NDB; ++j) {
+      qreg[2 * j] = load16(qrow + 32 * j + 16 * g);
+      qreg[2 * j + 1] = load16(qrow + 32 * j + 16 * g + 8);
+    }
+  }
+
+  uint8_t* ring = smem8c + kg * NST * 2 * C::kTile;
+  const uint32_t ring_lds = lds_address(ring);
+  int* info_page = reinterpret_cast<int*>(smem8c + C::kLds - C::kInfo);
+  int* info_slot = info_page + C::kThreads;
+  uint32_t* info_scale = reinterpret_cast<uint32_t*>(info_slot + C::kThreads);   // K | V << 16
+
+  f32x16 acc[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) acc[db] = f32x16{};
+  float m_run = -INFINITY, l_run = 0.f;
+  const float sl = GENERIC ? kLog2e : p.scale * kLog2e;
+
+  for (int s0 = k_begin; s0 < k_end; s0 += C::kSuper * BN) {
+    const int n_tiles = min((k_end - s0 + BN - 1) / BN, C::kSuper);
+    const int steps = (n_tiles + KG - 1) / KG;
+    // Pages and scales: thread i's 16-key group.
+    __syncthreads();   // the previous tiles' are done with (and the rings empty)
+    {
+      const int key = s0 + tid * 16;
+      int page = -1, slot = 0;
+      uint32_t sc = 127u | 127u << 16;
+      if (key < k_end) {
+        const int col = (int)fdiv(key, p.page);
+        slot = key - col * (int)p.page.d;
+        page = p.table != nullptr ? p.table[(int64_t)b * p.table_stride + col] : b;
+        if (page < 0 || page >= p.num_pages) {
+          page = -1;
+        } else {
+          const int blk = slot >> p.log2_block;
+          sc = (uint32_t)p.ks[page * p.ks_sp + blk * p.ks_sb + kvh * p.ks_sh] |
+               (uint32_t)p.vs[page * p.vs_sp + blk * p.vs_sb + kvh * p.vs_sh] << 16;
+        }
+      }
+      info_page[tid] = page;
+      info_slot[tid] = slot;
+      info_scale[tid] = sc;
+    }
+    __syncthreads();
+
+    // This wave's share of tile kg + KG * step into its stage.
+    auto issue = [&](int step) {
+      const int t = kg + KG * step;
+      const uint32_t st = ring_lds + (uint32_t)((step % NST) * 2 * C::kTile);
+      const int row_l = lane / CPR, pos = lane % CPR;
+#pragma unroll
+      for (int u = 0; u < GPW; ++u) {
+        const int gr = rw * GPW + u;
+        const int at = min(4 * t + gr, C::kThreads - 1);
+        const int page = t < n_tiles ? __builtin_amdgcn_readfirstlane(info_page[at]) : -1;
+        const int slot = __builtin_amdgcn_readfirstlane(info_slot[at]);
+        const int left = min(s.L - (s0 + t * BN + 16 * gr), 16);
+        const bool live = page >= 0 && left > 0;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const int64_t sp = kv ? p.v_sp : p.k_sp, ss = kv ? p.v_ss : p.k_ss, sh = kv ? p.v_sh : p.k_sh;
+          const uint8_t* base = kv ? p.v : p.k;
+          const u32x4 rs = make_rsrc_words(live ? base + page * sp + slot * ss + kvh * sh : base,
+                                           live ? (uint32_t)((left - 1) * ss + D) : 0u);
+#pragma unroll
+          for (int m = 0; m < IPG; ++m) {
+            const int in_group = m * RPI + row_l;   // (the swizzles repeat every 16 rows)
+            const int chunk = kv ? kv8_v_chunk<D>(in_group, pos) : kv8_k_chunk<D>(in_group, pos);
+            buf_load16_lds(rs, st + (uint32_t)(kv * C::kTile + (gr * IPG + m) * 1024),
+                           (uint32_t)(in_group * (int)ss + chunk * 16));
+          }
+        }
+      }
+    };
+
+    for (int i0 = 0; i0 < NST - 1; ++i0) issue(i0);
+#pragma unroll
+    for (int j = 0; j < 2 * NDB; ++j) asm volatile("" : "+v"(qreg[j]));
+    if (GENERIC) asm volatile("" : "+v"(row.slope));
+    for (int i0 = 0; i0 < steps; ++i0) {
+      // Tile i0 has landed, for every wave, and the stage that is filled next
+      // has been read.
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NST - 2) * PER) : "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      issue(i0 + NST - 1);
+      const int t = kg + KG * i0;
+      const int n0 = s0 + t * BN;
+      if (t >= n_tiles || n0 >= whi || n0 + BN <= wlo) continue;
+      const uint8_t* kt = ring + (i0 % NST) * 2 * C::kTile;
+      const uint8_t* vt = kt + C::kTile;
+      const bool masked = n0 < all_lo || n0 + BN - 1 > all_hi || n0 + BN > k_end;
+      f32x16 sc[2];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const float ksc = __uint_as_float((info_scale[4 * t + 2 * hf + (c32 >> 4)] & 0xffffu) << 23);
+        sc[hf] = kv8_qk<T, F8, D>(kt, 32 * hf, ksc, qreg);
+        if (GENERIC) kv8_score_options(p, row, n0 + 32 * hf, sc[hf]);
+        if (masked) kv8_mask(row, n0 + 32 * hf, sc[hf]);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[hf][v]);
+      }
+      mx = halves_max(mx) * sl;
+      const float m_new = fmaxf(m_run, mx);
+      if (__builtin_amdgcn_ballot_w64(m_new > m_run)) {
+        const float alpha = m_new == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+        l_run *= alpha;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) acc[db] *= alpha;
+        m_run = m_new;
+      }
+      const float m_use = m_run == -INFINITY ? 0.f : m_run;
+      const bool mixed = n0 < all_lo || (n0 + BN - 1 > all_hi && all_hi < s.L - 1);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        u32x4 pb[2];
+        kv8_exp<T>(sc[hf], sl, m_use, pb, l_run);
+        const float vsc[2] = {__uint_as_float(info_scale[4 * t + 2 * hf] >> 16 << 23),
+                              __uint_as_float(info_scale[4 * t + 2 * hf + 1] >> 16 << 23)};
+        kv8_pv<T, F8, D>(vt, 32 * hf, vsc, pb, sc[hf], mixed, acc);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+
+  // Merge the key groups: groups 1 .. KG - 1 leave their rows in LDS in the
+  // register order of the wave that takes them.
+  float l_w = halves_sum(l_run);
+  if constexpr (KG > 1) {
+    __syncthreads();
+    float* area = reinterpret_cast<float*>(smem8c);
+    if (kg > 0) {
+      float* to = area + ((kg - 1) * RW + rw) * (C::kWave / 4);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+          *reinterpret_cast<f32x4*>(to + ((db * 4 + q4) * 64 + lane) * 4) =
+              f32x4{acc[db][4 * q4], acc[db][4 * q4 + 1], acc[db][4 * q4 + 2], acc[db][4 * q4 + 3]};
+      if (g == 0) {
+        to[32 * D + 2 * c32] = m_run;
+        to[32 * D + 2 * c32 + 1] = l_w;
+      }
+    }
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int u = 1; u < KG; ++u) {
+      const float* from = area + ((u - 1) * RW + rw) * (C::kWave / 4);
+      const float mu = from[32 * D + 2 * c32], lu = from[32 * D + 2 * c32 + 1];
+      const float m_new = fmaxf(m_run, mu);
+      // (a group without keys has l = 0; a NaN sum stays one)
+      const float a0 = l_w != 0.f ? __builtin_amdgcn_exp2f(m_run - m_new) : 0.f;
+      const float a1 = lu != 0.f ? __builtin_amdgcn_exp2f(mu - m_new) : 0.f;
+      l_w = l_w * a0 + lu * a1;
+      m_run = m_new;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(from + ((db * 4 + q4) * 64 + lane) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[db][4 * q4 + e] = acc[db][4 * q4 + e] * a0 + x[e] * a1;
+        }
+    }
+  }
+  if (!row_valid) return;
+  const float inv = l_w == 0.f ? 0.f : 1.f / l_w;
+  if (p.chunk_splits == 1) {
+    uint16_t* dst = static_cast<uint16_t*>(p.o) + kv8_base(p, s, p.o_sb, p.o_ss) + (int64_t)qi * p.o_ss +
+                    (int64_t)head * p.o_sh;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        *reinterpret_cast<u32x2*>(dst + 32 * db + 8 * q4 + 4 * g) =
+            u32x2{T::pack2(acc[db][4 * q4] * inv, acc[db][4 * q4 + 1] * inv),
+                  T::pack2(acc[db][4 * q4 + 2] * inv, acc[db][4 * q4 + 3] * inv)};
+  } else {
+    const int64_t prow = ((int64_t)split * p.total_q + kv8_out_row(p, s, qi)) * p.heads_q + head;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        *reinterpret_cast<f32x4*>(p.o_part + prow * D + 32 * db + 8 * q4 + 4 * g) =
+            f32x4{acc[db][4 * q4] * inv, acc[db][4 * q4 + 1] * inv, acc[db][4 * q4 + 2] * inv,
+                  acc[db][4 * q4 + 3] * inv};
+    if (g == 0) p.lse_part[prow] = l_w == 0.f ? -INFINITY : m_run + __log2f(l_w);
+  }
+}
+
 // Merges the splits of each row: out = sum_s 2^(lse_s - lse) o_s over the
 // splits that hold keys its workgroup saw (the others are unwritten).  One
 // thread per row and 4 dims, a workgroup within one sequence; partials are
@@ -519,12 +863,16 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(const Kv8AttnParams p)
   if (item >= (int64_t)s.n * p.heads_q) return;
   const int qd = (int)(idx % kQuads), h = (int)(item % p.heads_q), i = (int)(item / p.heads_q);
   const int G = (int)p.group.d;
-  // The splits that the row's 32-row block ran: those that meet its keys.
-  const int rb = (i * G + h % G) / 32, last = min(rb * 32 + 31, s.n * G - 1);
+  // The splits that the row's workgroups ran: those that meet their keys.
+  const bool chunk = s.n * G > kKv8SplitRows;
+  const int splits = chunk ? p.chunk_splits : p.num_splits, keys = chunk ? p.chunk_keys : p.split_keys;
+  if (splits == 1) return;   // (written by the row's only workgroup)
+  const int bm = chunk ? p.chunk_rows : kKv8SplitRows;
+  const int rb = (i * G + h % G) / bm, last = min(rb * bm + bm - 1, s.n * G - 1);
   int lo, hi;
-  kv8_key_range(p, s, (int)fdiv(rb * 32, p.group), (int)fdiv(last, p.group), lo, hi);
-  const int s_lo = lo / p.split_keys;
-  const int n = hi > lo ? min(p.num_splits, (hi + p.split_keys - 1) / p.split_keys) : 0;
+  kv8_key_range(p, s, (int)fdiv(rb * bm, p.group), (int)fdiv(last, p.group), lo, hi);
+  const int s_lo = lo / keys;
+  const int n = hi > lo ? min(splits, (hi + keys - 1) / keys) : 0;
   const int64_t row = kv8_out_row(p, s, i) * p.heads_q + h, step = p.total_q * p.heads_q;
   float m = -INFINITY, tot = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -567,18 +915,31 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(const Kv8AttnParams p)
 }
 
 template <class T, class F8, int D, bool GENERIC>
-hipError_t launch_kv8_split(const Kv8AttnParams& p, hipStream_t st) {
-  constexpr int NST = D == 256 ? 2 : D == 128 ? 2 : 4;
-  using Tile = Kv8Tile<D, NST>;
-  auto kern = kv8_split_kernel<T, F8, D, NST, GENERIC>;
-  static std::atomic<uint64_t> lds_devices{0};
-  if (hipError_t e = set_lds_limit(lds_devices, kern, Tile::kLds); e != hipSuccess) return e;
-  const int64_t wgs = (int64_t)p.num_splits * p.batch * p.row_blocks * p.heads_k;
-  if (wgs <= 0) return hipSuccess;
-  if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(kKv8Waves * 64), Tile::kLds, st, p);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.num_splits == 1) return e;
+hipError_t launch_kv8(const Kv8AttnParams& p, hipStream_t st) {
+  if (p.num_splits > 0) {
+    constexpr int NST = D == 64 ? 4 : 2;
+    using Tile = Kv8Tile<D, NST>;
+    auto kern = kv8_split_kernel<T, F8, D, NST, GENERIC>;
+    static std::atomic<uint64_t> lds_devices{0};
+    if (hipError_t e = set_lds_limit(lds_devices, kern, Tile::kLds); e != hipSuccess) return e;
+    const int64_t wgs = (int64_t)p.num_splits * p.batch * p.heads_k;
+    if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(kKv8Waves * 64), Tile::kLds, st, p);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  if (p.chunk_splits > 0) {
+    // D = 256: one wave per SIMD has the registers for a row's sums.
+    constexpr int RW = kKv8ChunkRows / 32, KG = D == 256 ? 1 : 2, NST = 3;
+    using C = Kv8Chunk<D, RW, KG, NST>;
+    auto kern = kv8_chunk_kernel<T, F8, D, RW, KG, NST, GENERIC>;
+    static std::atomic<uint64_t> lds_devices{0};
+    if (hipError_t e = set_lds_limit(lds_devices, kern, C::kLds); e != hipSuccess) return e;
+    const int64_t wgs = (int64_t)p.chunk_splits * p.chunk_blocks * p.batch * p.heads_k;
+    if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(C::kThreads), C::kLds, st, p);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  if (p.num_splits <= 1 && p.chunk_splits <= 1) return hipSuccess;
   const int64_t threads = (int64_t)p.seqlen_q * p.heads_q * (D / 4);
   hipLaunchKernelGGL((kv8_combine_kernel<T, D>), dim3((unsigned)((threads + 255) / 256), (unsigned)p.batch),
                      dim3(256), 0, st, p);
@@ -588,8 +949,7 @@ hipError_t launch_kv8_split(const Kv8AttnParams& p, hipStream_t st) {
 template <class T>
 hipError_t launch_kv8_attn(int store, const Kv8AttnParams& p, int head_dim, hipStream_t st) {
   const bool generic = p.alibi != nullptr || p.softcap > 0.f || !(p.scale > 0.f);
-#define FA_KV8(FF, DD)                                                     \
-  return generic ? launch_kv8_split<T, FF, DD, true>(p, st) : launch_kv8_split<T, FF, DD, false>(p, st);
+#define FA_KV8(FF, DD) return generic ? launch_kv8<T, FF, DD, true>(p, st) : launch_kv8<T, FF, DD, false>(p, st);
 #define FA_KV8_D(FF)                      \
   if (head_dim == 64) { FA_KV8(FF, 64) }   \
   if (head_dim == 128) { FA_KV8(FF, 128) } \

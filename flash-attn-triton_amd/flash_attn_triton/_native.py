@@ -92,11 +92,11 @@ _SIGNATURES = {
                                 _vp, _vp, _vp, _vp]),
     "fa_kvcache8_append": (_int, [_vp, _vp, _i64p, _i64p, _int, _vp, _vp, _i64p, _i64p, _int, _vp, _vp,
                                   _i64p, _i64p, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
-    "fa_fwd_kvcache8_plan": (_int, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32p, _i64p]),
+    "fa_fwd_kvcache8_plan": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64p]),
     "fa_fwd_kvcache8": (_int, [_vp, _vp, _i64p, _i64p, _int, _vp, _vp, _i64p, _i64p, _int, _vp, _vp,
                                _i64p, _i64p, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64,
                                _i64, _i64, _i64, _i64, _i64, _f32, _int, _i64, _i64, _f32, _vp, _i64,
-                               _i32, _vp, _i64, _vp]),
+                               _vp, _i64, _vp]),
     "fa_quant_k_int8": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64p, _vp]),
     "fa_fwd_int8": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64p, _i64p,
                            _i64p, _f32, _int, _i64, _i64, _vp]),
@@ -498,12 +498,13 @@ def kvcache8_append(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapping) -> N
 
 
 @functools.lru_cache(maxsize=1024)
-def kvcache8_plan(batch: int, max_seqlen_q: int, total_q: int, heads_q: int, heads_k: int, head_dim: int,
-                  max_keys: int):
-    splits, ws = ctypes.c_int32(0), ctypes.c_int64(0)
-    _check(load().fa_fwd_kvcache8_plan(batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys,
-                                       ctypes.byref(splits), ctypes.byref(ws)), "fa_fwd_kvcache8_plan")
-    return int(splits.value), int(ws.value)
+def kvcache8_plan(packed: bool, batch: int, max_seqlen_q: int, total_q: int, heads_q: int, heads_k: int,
+                  head_dim: int, max_keys: int) -> int:
+    """Workspace bytes of fwd_kvcache8."""
+    ws = ctypes.c_int64(0)
+    _check(load().fa_fwd_kvcache8_plan(packed, batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys,
+                                       ctypes.byref(ws)), "fa_fwd_kvcache8_plan")
+    return int(ws.value)
 
 
 def fwd_kvcache8(q, out, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, cu_seqlens_q,
@@ -515,7 +516,7 @@ def fwd_kvcache8(q, out, k_cache, v_cache, k_scale, v_scale, cache_seqlens, bloc
     pages, page, Hk = k_cache.shape[:3]
     packed = cu_seqlens_q is not None
     total = q.shape[0] if packed else batch * max_seqlen_q
-    splits, ws_bytes = kvcache8_plan(batch, max_seqlen_q, total, Hq, Hk, D, max_keys)
+    ws_bytes = kvcache8_plan(packed, batch, max_seqlen_q, total, Hq, Hk, D, max_keys)
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     qs, os_ = q.stride(), out.stride()
     q_stride = _strides((0,) + qs[:2] if packed else qs[:3])
@@ -528,7 +529,7 @@ def fwd_kvcache8(q, out, k_cache, v_cache, k_scale, v_scale, cache_seqlens, bloc
         _ptr(cache_seqlens), _ptr(block_table), block_table.stride(0) if tabled else 0,
         block_table.shape[1] if tabled else 0, pages, page, page // k_scale.shape[1], _ptr(cu_seqlens_q),
         batch, max_seqlen_q, total, max_keys, Hq, Hk, D, softmax_scale, int(bool(causal)), window_left,
-        window_right, softcap, _ptr(alibi), alibi.stride(0) if alibi is not None else 0, splits,
+        window_right, softcap, _ptr(alibi), alibi.stride(0) if alibi is not None else 0,
         _ptr(workspace), ws_bytes, _stream(q.device))
     _check(status, "fa_fwd_kvcache8")
 

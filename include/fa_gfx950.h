@@ -469,10 +469,10 @@ int fa_kvcache8_append(const void* k, const void* v, const int64_t* k_stride, co
                        int64_t page_size, int64_t block, int64_t heads_k, int64_t head_dim,
                        fa_stream_t stream);
 
-/* Splits of the keys and bytes of workspace (fp32 partial rows) of
- * fa_fwd_kvcache8.  Host only. */
-int fa_fwd_kvcache8_plan(int64_t batch, int64_t max_seqlen_q, int64_t total_q, int64_t heads_q,
-                         int64_t heads_k, int64_t head_dim, int64_t max_keys, int32_t* num_splits,
+/* Bytes of workspace (fp32 partial rows of the key splits) of fa_fwd_kvcache8
+ * for these sizes; packed: with cu_seqlens_q.  Host only. */
+int fa_fwd_kvcache8_plan(int packed, int64_t batch, int64_t max_seqlen_q, int64_t total_q,
+                         int64_t heads_q, int64_t heads_k, int64_t head_dim, int64_t max_keys,
                          int64_t* workspace_bytes);
 
 /* Attention of queries against the 8-bit cache: fa_fwd_kvcache with q and out
@@ -488,7 +488,8 @@ int fa_fwd_kvcache8_plan(int64_t batch, int64_t max_seqlen_q, int64_t total_q, i
  * fa_fwd_varlen.  Rows of packed q outside every sequence are not written.
  * Whatever the device arrays hold nothing outside the tensors is read or
  * written: a page outside the cache reads as zeros, a sequence whose offsets
- * leave q has no queries.  num_splits and workspace come from the plan. */
+ * leave q has no queries.  workspace (NULL if the plan says 0) belongs to the
+ * call until the stream has passed it. */
 int fa_fwd_kvcache8(const void* q, void* out, const int64_t* q_stride, const int64_t* o_stride, int dtype,
                     const void* k_cache, const void* v_cache, const int64_t* k_cache_stride,
                     const int64_t* v_cache_stride, int store, const uint8_t* k_scale,
@@ -499,8 +500,8 @@ int fa_fwd_kvcache8(const void* q, void* out, const int64_t* q_stride, const int
                     int64_t batch, int64_t max_seqlen_q, int64_t total_q, int64_t max_keys,
                     int64_t heads_q, int64_t heads_k, int64_t head_dim, float softmax_scale, int causal,
                     int64_t window_left, int64_t window_right, float softcap, const float* alibi_slopes,
-                    int64_t alibi_batch_stride, int32_t num_splits, void* workspace,
-                    int64_t workspace_bytes, fa_stream_t stream);
+                    int64_t alibi_batch_stride, void* workspace, int64_t workspace_bytes,
+                    fa_stream_t stream);
 
 /* Per-token INT8 quantization of K (fp16), bit-exact with
  * `_quantize_k_rows` (attention_kernel_int8.py:58-79, launched at :232):

@@ -108,19 +108,20 @@ def test_c_attention_checks(lib):
     one, st = ctypes.c_void_p(16), _native._strides((4096, 1024, 64))
 
     def call(q=one, dtype=0, store=0, table=one, cols=4, pages=8, page=32, block=16, cu=None, batch=2, max_q=1, total=2,
-             max_keys=128, hq=2, hk=1, dim=64, splits=None, ws=one, kst=st, softcap=0.0):
-        n, need = ctypes.c_int32(0), ctypes.c_int64(0)
-        lib.fa_fwd_kvcache8_plan(batch, max_q, total, hq, hk, dim, max_keys, ctypes.byref(n), ctypes.byref(need))
+             max_keys=128, hq=2, hk=1, dim=64, less=0, ws=one, kst=st, softcap=0.0):
+        need = ctypes.c_int64(0)
+        lib.fa_fwd_kvcache8_plan(0, batch, max_q, total, hq, hk, dim, max_keys, ctypes.byref(need))
         return lib.fa_fwd_kvcache8(q, one, st, st, dtype, one, one, kst, kst, store, one, one, st, st, one, table, 4, cols,
                                    pages, page, block, cu, batch, max_q, total, max_keys, hq, hk, dim, 1.0, 1, -1, -1,
-                                   softcap, None, 0, n.value if splits is None else splits, ws, need.value, None)
+                                   softcap, None, 0, ws, need.value - less, None)
     assert call(q=None) == _native.FA_ERR_INVALID
     assert call(dtype=2) == _native.FA_ERR_UNSUPPORTED
     assert call(max_keys=129) == _native.FA_ERR_INVALID and "block table" in _error(lib)
     assert call(table=None, max_keys=33) == _native.FA_ERR_INVALID
     assert call(total=3) == _native.FA_ERR_INVALID
     assert call(hq=3, hk=2) == _native.FA_ERR_INVALID
-    assert call(splits=7) == _native.FA_ERR_INVALID and "plan" in _error(lib)
+    assert call(cols=40, max_keys=1280, less=4) == _native.FA_ERR_INVALID and "plan" in _error(lib)
+    assert call(cols=40, max_keys=1280, ws=None) == _native.FA_ERR_INVALID
     assert call(softcap=-1.0) == _native.FA_ERR_INVALID
     assert call(softcap=math.nan) == _native.FA_ERR_INVALID
     assert call(kst=_native._strides((4096, 32, 64))) == _native.FA_ERR_UNSUPPORTED and "overlap" in _error(lib)
@@ -128,11 +129,12 @@ def test_c_attention_checks(lib):
     assert call(batch=0, total=0) == _native.FA_OK
 
 
-def test_plan_holds_every_partial(lib):
-    for args in ((1, 1, 1, 32, 8, 128, 131001), (64, 1, 64, 32, 8, 128, 8192), (3, 700, 900, 16, 4, 64, 4000)):
-        n, need = ctypes.c_int32(0), ctypes.c_int64(0)
-        assert lib.fa_fwd_kvcache8_plan(*args, ctypes.byref(n), ctypes.byref(need)) == _native.FA_OK
-        assert n.value >= 1 and need.value == (n.value * args[2] * args[3] * (args[5] + 1) * 4 if n.value > 1 else 0)
+def test_plan_asks_for_whole_rows(lib):
+    # fp32 rows and a sum for every split of every row of q
+    for args in ((0, 1, 1, 1, 32, 8, 128, 131001), (0, 64, 1, 64, 32, 8, 128, 8192), (1, 3, 700, 900, 16, 4, 64, 4000)):
+        need = ctypes.c_int64(0)
+        assert lib.fa_fwd_kvcache8_plan(*args, ctypes.byref(need)) == _native.FA_OK
+        assert need.value > 0 and need.value % (args[3] * args[4] * (args[6] + 1) * 4) == 0
 
 
 def test_scale_rule():
