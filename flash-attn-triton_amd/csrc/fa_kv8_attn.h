@@ -31,6 +31,8 @@
 // with a product of indicators.
 #pragma once
 
+#include <type_traits>
+
 #include "fa_common.h"
 #include "fa_kv8.h"
 
@@ -38,6 +40,7 @@ namespace fa {
 
 constexpr int kKv8Waves = 4;
 constexpr int kKv8BN = 32;            // keys of a tile
+constexpr float kKv8Slack = 8.f;      // a maximum is raised by more than this (log2 units) or not at all
 static_assert(kKv8MaxSplit == 32 * kKv8Waves * kKv8BN, "64 lanes hold the 16-key groups of 32 tiles");
 
 // The 8-bit types.  bad(): the high bit of each byte of a word whose number is
@@ -151,7 +154,9 @@ __device__ inline void kv8_key_range(const Kv8AttnParams& p, const Kv8Rows& s, i
 
 // What a query row of a lane sees and how its scores are scaled.
 struct Kv8Row {
-  int key_lo, key_hi, qpos;
+  int key_lo;
+  uint32_t keys;   // sees key_lo .. key_lo + keys
+  int qpos;
   float slope;
 };
 
@@ -159,28 +164,55 @@ template <bool GENERIC>
 __device__ inline Kv8Row kv8_row(const Kv8AttnParams& p, const Kv8Rows& s, int qi, int head, int k_end) {
   Kv8Row r;
   r.qpos = qi + (p.causal ? s.L - s.n : 0);
-  r.key_lo = 0;
-  r.key_hi = k_end - 1;   // (the workgroup's keys end there)
-  if (p.causal) r.key_hi = min(r.key_hi, r.qpos);
-  if (p.window_right >= 0) r.key_hi = min(r.key_hi, r.qpos + p.window_right);
-  if (p.window_left >= 0) r.key_lo = max(0, r.qpos - p.window_left);
+  int lo = 0, hi = k_end - 1;   // (the workgroup's keys end there)
+  if (p.causal) hi = min(hi, r.qpos);
+  if (p.window_right >= 0) hi = min(hi, r.qpos + p.window_right);
+  if (p.window_left >= 0) lo = max(0, r.qpos - p.window_left);
+  r.key_lo = hi >= lo ? lo : 1 << 30;   // none: past every key
+  r.keys = hi >= lo ? (uint32_t)(hi - lo) : 0;
   r.slope = GENERIC && p.alibi != nullptr ? p.alibi[(int64_t)s.b * p.alibi_sb + head] : 0.f;
   return r;
 }
 
-// S^T of 32 keys: LDS rows row0 .. row0 + 31 of a K tile against Q^T in
-// registers, the rows scaled by ksc (one value per lane: its key's).
-template <class T, class F8, int D>
-__device__ inline f32x16 kv8_qk(const uint8_t* kt, int row0, float ksc, const u32x4* qreg) {
-  const int lane = threadIdx.x & 63, row = row0 + (lane & 31), g = lane >> 5;
-  f32x16 sc = f32x16{};
+// Byte offsets of a lane's operand reads in a tile of 32 keys (the swizzles
+// repeat every 16 rows, so the other steps and halves are constants away).  K:
+// row lane % 32, chunk 2 j + lane / 32.  V: the lane's 8 keys of 16-key step cc
+// are 16 cc + 4 g + {0..3, 8..11}; lane i of 16 names 8 bytes of row i / 2.
+template <int D>
+struct Kv8Lane {
+  uint32_t k[D / 32], v[D / 32];
+  __device__ inline Kv8Lane() {
+    const int lane = threadIdx.x & 63, c32 = lane & 31, g = lane >> 5;
+    const int vr = (lane & 15) >> 1, vkey = 4 * g + (vr & 3) + 8 * (vr >> 2);
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j) {
-    const u32x4 raw = load16(kt + row * D + kv8_k_chunk<D>(row, 2 * j + g) * 16);
-    sc = T::mfma32(kv8_operand<T, F8>(raw[0], raw[1], ksc), qreg[2 * j], sc);
-    sc = T::mfma32(kv8_operand<T, F8>(raw[2], raw[3], ksc), qreg[2 * j + 1], sc);
+    for (int j = 0; j < D / 32; ++j) {
+      k[j] = (uint32_t)(c32 * D + kv8_k_chunk<D>(c32, 2 * j + g) * 16);
+      v[j] = (uint32_t)(vkey * D + kv8_v_chunk<D>(vkey, 2 * j + ((lane >> 4) & 1)) * 16 + 8 * (lane & 1));
+    }
   }
-  return sc;
+};
+
+// S^T of NH x 32 keys: the rows of a K tile in LDS against Q^T in registers,
+// each row scaled by its key's ksc[h].  Every operand is read before the first
+// product, and the products of the halves take turns: neither an LDS read nor
+// the chain of one accumulator is waited for in between.
+template <class T, class F8, int D, int NH>
+__device__ inline void kv8_qk(const uint8_t* kt, const Kv8Lane<D>& at, const float* ksc, const u32x4* qreg,
+                              f32x16* sc) {
+  u32x4 raw[NH][D / 32];
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+    for (int h = 0; h < NH; ++h) raw[h][j] = load16(kt + at.k[j] + 32 * h * D);
+#pragma unroll
+  for (int h = 0; h < NH; ++h) sc[h] = f32x16{};
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+        sc[h] = T::mfma32(kv8_operand<T, F8>(raw[h][j][2 * u], raw[h][j][2 * u + 1], ksc[h]), qreg[2 * j + u], sc[h]);
 }
 
 // Scale, ALiBi and softcap of the scores of keys n0 .. n0 + 31.
@@ -205,7 +237,7 @@ __device__ inline void kv8_mask(const Kv8Row& row, int n0, f32x16& sc) {
 #pragma unroll
   for (int v = 0; v < 16; ++v) {
     const int key = n0 + 8 * (v >> 2) + 4 * g + (v & 3);
-    if (key < row.key_lo || key > row.key_hi) sc[v] = -INFINITY;
+    sc[v] = (uint32_t)(key - row.key_lo) > row.keys ? -INFINITY : sc[v];
   }
 }
 
@@ -224,26 +256,18 @@ __device__ inline void kv8_exp(const f32x16& sc, float sl, float m, u32x4* pb, f
     }
 }
 
-// O^T += V^T P^T over the 32 keys of LDS rows row0 .. of a V tile, scaled by
-// vsc (16 keys each).  mixed: the rows of the wave do not all see all of these
-// keys, and a V number that is not finite must not meet a P of 0.
+// O^T += V^T P^T over the 32 keys of V in LDS from row0 on, scaled by vsc (16
+// keys each).  mixed: the rows of the wave do not all see all of these keys, and
+// a V number that is not finite must not meet a P of 0.
 template <class T, class F8, int D>
-__device__ inline void kv8_pv(const uint8_t* vt, int row0, const float* vsc, const u32x4* pb,
-                              const f32x16& sc, bool mixed, f32x16* acc) {
+__device__ inline void kv8_pv(const uint8_t* vt, const Kv8Lane<D>& at, int row0, const float* vsc,
+                              const u32x4* pb, const f32x16& sc, bool mixed, f32x16* acc) {
   constexpr int NDB = D / 32;
-  const int lane = threadIdx.x & 63, g = lane >> 5;
-  // The lane's 8 keys of step cc are 16 cc + 4 g + {0..3, 8..11}: row i / 2 of
-  // the transposed read, i the lane among its 16.
-  const int vr = (lane & 15) >> 1, vkey = 4 * g + (vr & 3) + 8 * (vr >> 2);
-  const int vc = (lane >> 4) & 1, vh = 8 * (lane & 1);
   u32x2 raw[2][NDB];
 #pragma unroll
   for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
-    for (int db = 0; db < NDB; ++db) {
-      const int row = row0 + 16 * cc + vkey;
-      raw[cc][db] = lds_read_tr8(vt + row * D + kv8_v_chunk<D>(row, 2 * db + vc) * 16 + vh);
-    }
+    for (int db = 0; db < NDB; ++db) raw[cc][db] = lds_read_tr8(vt + at.v[db] + (row0 + 16 * cc) * D);
   if (mixed) {
     uint32_t flags = 0;
 #pragma unroll
@@ -252,14 +276,17 @@ __device__ inline void kv8_pv(const uint8_t* vt, int row0, const float* vsc, con
       for (int db = 0; db < NDB; ++db) flags |= F8::bad(raw[cc][db][0]) | F8::bad(raw[cc][db][1]);
     if (__builtin_amdgcn_ballot_w64(flags != 0) != 0) {
       // Visible (key, row) pairs and numbers that are not finite, as 1 and 0: a
-      // row gets NaN in the columns where their product is not zero.
+      // row gets NaN (all bits set) in the columns where their product is not
+      // zero.  In integer operations: comparisons would take a pair of scalar
+      // registers each, which the loop around this has no room for.
+      const uint32_t one = std::is_same<T, F16>::value ? 0x3c00u : 0x3f80u;
+      auto seen1 = [&](float x) { return min(__float_as_uint(x) ^ 0xff800000u, 1u) * one; };   // not -inf
       u32x4 seen[2];
 #pragma unroll
       for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          seen[cc][j] = T::pack2(sc[cc * 8 + 2 * j] == -INFINITY ? 0.f : 1.f,
-                                 sc[cc * 8 + 2 * j + 1] == -INFINITY ? 0.f : 1.f);
+          seen[cc][j] = seen1(sc[cc * 8 + 2 * j]) | seen1(sc[cc * 8 + 2 * j + 1]) << 16;
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
         f32x16 hit = f32x16{};
@@ -268,16 +295,17 @@ __device__ inline void kv8_pv(const uint8_t* vt, int row0, const float* vsc, con
           u32x4 ind;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const uint32_t f = F8::bad(raw[cc][db][e]);
-            ind[2 * e] = T::pack2((f & 0x80u) ? 1.f : 0.f, (f & 0x8000u) ? 1.f : 0.f);
-            ind[2 * e + 1] = T::pack2((f & 0x800000u) ? 1.f : 0.f, (f & 0x80000000u) ? 1.f : 0.f);
-            raw[cc][db][e] &= ~((f >> 7) * 0xffu);
+            const uint32_t f = F8::bad(raw[cc][db][e]) >> 7;   // a bit per byte
+            ind[2 * e] = (f & 1u) * one | ((f >> 8) & 1u) * one << 16;
+            ind[2 * e + 1] = ((f >> 16) & 1u) * one | (f >> 24) * one << 16;
+            raw[cc][db][e] &= ~(f * 0xffu);
           }
           hit = T::mfma32(ind, seen[cc], hit);
         }
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-          if (hit[v] > 0.f) acc[db][v] = __uint_as_float(0x7fc00000u);
+          acc[db][v] = __uint_as_float(__float_as_uint(acc[db][v]) |
+                                       (uint32_t)(-(int)__float_as_uint(hit[v]) >> 31));
       }
     }
   }
@@ -286,6 +314,22 @@ __device__ inline void kv8_pv(const uint8_t* vt, int row0, const float* vsc, con
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
       acc[db] = T::mfma32(kv8_operand<T, F8>(raw[cc][db][0], raw[cc][db][1], vsc[cc]), pb[cc], acc[db]);
+}
+
+// Raises the running maximum m (log2 units) of rows whose new one passes it by
+// more than kKv8Slack, and rescales their sums: P then stays below 2^8, and
+// most tiles leave the output alone.
+template <int NDB>
+__device__ inline void kv8_raise(float mx, float& m, float& l, f32x16* acc) {
+  const bool raise = mx > m + kKv8Slack;
+  if (__builtin_amdgcn_ballot_w64(raise)) {
+    const float m_new = raise ? mx : m;
+    const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+    l *= alpha;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) acc[db] *= alpha;
+    m = m_new;
+  }
 }
 
 template <int D, int NST>
@@ -414,6 +458,7 @@ void kv8_split_kernel(const Kv8AttnParams p) {
     }
   };
 
+  const Kv8Lane<D> at;
   f32x16 acc[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) acc[db] = f32x16{};
@@ -441,21 +486,16 @@ void kv8_split_kernel(const Kv8AttnParams p) {
 
     const float ks0 = __uint_as_float(__builtin_amdgcn_readlane(ks_l, 2 * t));
     const float ks1 = __uint_as_float(__builtin_amdgcn_readlane(ks_l, 2 * t + 1));
-    f32x16 sc = kv8_qk<T, F8, D>(kt, 0, c32 < 16 ? ks0 : ks1, qreg);
+    const float ksc = c32 < 16 ? ks0 : ks1;
+    f32x16 sc;
+    kv8_qk<T, F8, D, 1>(kt, at, &ksc, qreg, &sc);
     if (GENERIC) kv8_score_options(p, row, n0, sc);
     if (n0 < all_lo || n0 + BN - 1 > all_hi) kv8_mask(row, n0, sc);
     float mx = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[v]);
+    for (int v = 0; v < 16; v += 2) mx = fmaxf(mx, fmaxf(sc[v], sc[v + 1]));
     mx = halves_max(mx) * sl;
-    const float m_new = fmaxf(m_run, mx);
-    if (__builtin_amdgcn_ballot_w64(m_new > m_run)) {
-      const float alpha = m_new == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
-      l_run *= alpha;
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) acc[db] *= alpha;
-      m_run = m_new;
-    }
+    kv8_raise<NDB>(mx, m_run, l_run, acc);
     u32x4 pb[2];
     kv8_exp<T>(sc, sl, m_run == -INFINITY ? 0.f : m_run, pb, l_run);
 
@@ -465,7 +505,7 @@ void kv8_split_kernel(const Kv8AttnParams p) {
                           __uint_as_float(__builtin_amdgcn_readlane(vs_l, 2 * t + 1))};
     // (keys past the sequence's end are zeros in V)
     const bool mixed = n0 < all_lo || (n0 + BN - 1 > all_hi && all_hi < s.L - 1);
-    kv8_pv<T, F8, D>(vt, 0, vsc, pb, sc, mixed, acc);
+    kv8_pv<T, F8, D>(vt, at, 0, vsc, pb, sc, mixed, acc);
   }
 
   // ------------------------------------------------------------ merge waves
@@ -668,6 +708,7 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
   int* info_slot = info_page + C::kThreads;
   uint32_t* info_scale = reinterpret_cast<uint32_t*>(info_slot + C::kThreads);   // K | V << 16
 
+  const Kv8Lane<D> at;
   f32x16 acc[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) acc[db] = f32x16{};
@@ -750,24 +791,18 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
       const bool masked = n0 < all_lo || n0 + BN - 1 > all_hi || n0 + BN > k_end;
       f32x16 sc[2];
       float mx = -INFINITY;
+      const float ksc[2] = {__uint_as_float((info_scale[4 * t + (c32 >> 4)] & 0xffffu) << 23),
+                            __uint_as_float((info_scale[4 * t + 2 + (c32 >> 4)] & 0xffffu) << 23)};
+      kv8_qk<T, F8, D, 2>(kt, at, ksc, qreg, sc);
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const float ksc = __uint_as_float((info_scale[4 * t + 2 * hf + (c32 >> 4)] & 0xffffu) << 23);
-        sc[hf] = kv8_qk<T, F8, D>(kt, 32 * hf, ksc, qreg);
         if (GENERIC) kv8_score_options(p, row, n0 + 32 * hf, sc[hf]);
         if (masked) kv8_mask(row, n0 + 32 * hf, sc[hf]);
 #pragma unroll
-        for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[hf][v]);
+        for (int v = 0; v < 16; v += 2) mx = fmaxf(mx, fmaxf(sc[hf][v], sc[hf][v + 1]));
       }
       mx = halves_max(mx) * sl;
-      const float m_new = fmaxf(m_run, mx);
-      if (__builtin_amdgcn_ballot_w64(m_new > m_run)) {
-        const float alpha = m_new == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
-        l_run *= alpha;
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) acc[db] *= alpha;
-        m_run = m_new;
-      }
+      kv8_raise<NDB>(mx, m_run, l_run, acc);
       const float m_use = m_run == -INFINITY ? 0.f : m_run;
       const bool mixed = n0 < all_lo || (n0 + BN - 1 > all_hi && all_hi < s.L - 1);
 #pragma unroll
@@ -776,7 +811,7 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
         kv8_exp<T>(sc[hf], sl, m_use, pb, l_run);
         const float vsc[2] = {__uint_as_float(info_scale[4 * t + 2 * hf] >> 16 << 23),
                               __uint_as_float(info_scale[4 * t + 2 * hf + 1] >> 16 << 23)};
-        kv8_pv<T, F8, D>(vt, 32 * hf, vsc, pb, sc[hf], mixed, acc);
+        kv8_pv<T, F8, D>(vt, at, 32 * hf, vsc, pb, sc[hf], mixed, acc);
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
