@@ -59,11 +59,12 @@ struct Kv8AttnParams {
   float scale, softcap;
   const float* alibi; int64_t alibi_sb;
   int causal, window_left, window_right;
-  // Sequences of at most 32 rows (queries times the group) per K/V head:
-  // kv8_split_kernel, their keys in num_splits splits of split_keys (0: there are
-  // none).  The others: kv8_chunk_kernel, chunk_blocks blocks of chunk_rows rows.
+  // Launches whose sequences have at most 32 rows (queries times the group) per
+  // K/V head: kv8_split_kernel, the keys in num_splits splits of split_keys.  The
+  // others: kv8_chunk_kernel, chunk_blocks blocks of rows in all (at least).
+  // The splits of the kernel that is not launched are 0.
   int split_keys, num_splits;
-  int chunk_rows, chunk_blocks, chunk_keys, chunk_splits;
+  int chunk_blocks, chunk_keys, chunk_splits;
   float* o_part; float* lse_part;   // [split][row of q][head](D); LSE in log2 units
 };
 

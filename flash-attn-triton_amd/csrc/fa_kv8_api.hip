@@ -74,13 +74,13 @@ struct Plan {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How the keys are split.  Packed queries may hold sequences for both kernels;
-// the host only knows the longest.
-Plan make_plan(bool packed, int64_t batch, int64_t seqlen_q, int64_t total_q, int64_t heads_q,
-               int64_t heads_k, int64_t head_dim, int64_t max_keys) {
+// Which kernel takes the launch and how the keys are split.
+Plan make_plan(int64_t batch, int64_t seqlen_q, int64_t total_q, int64_t heads_q, int64_t heads_k,
+               int64_t head_dim, int64_t max_keys) {
   Plan pl = {};
   const int64_t group = heads_q / heads_k, rows = seqlen_q * group;
-  if (packed || rows <= fa::kKv8SplitRows) {
+  max_keys = max_keys > 0 ? max_keys : 1;
+  if (rows <= fa::kKv8SplitRows) {
     // The largest of 4096 .. 256 keys that leaves every CU several workgroups,
     // else 128 (a tile per wave).
     pl.split_keys = 128;
@@ -89,17 +89,17 @@ Plan make_plan(bool packed, int64_t batch, int64_t seqlen_q, int64_t total_q, in
         pl.split_keys = sk;
         break;
       }
-    pl.num_splits = (int)ceil_div(max_keys > 0 ? max_keys : 1, pl.split_keys);
-  }
-  if (rows > fa::kKv8SplitRows) {
-    pl.chunk_blocks = (int)ceil_div(rows, fa::kKv8ChunkRows);
-    const int64_t most = batch * pl.chunk_blocks, by_rows = ceil_div(total_q * group, fa::kKv8ChunkRows) + batch;
-    const int64_t wgs = heads_k * (most < by_rows ? most : by_rows);
+    pl.num_splits = (int)ceil_div(max_keys, pl.split_keys);
+  } else {
+    const int64_t most = batch * ceil_div(rows, fa::kKv8ChunkRows);
+    const int64_t by_rows = total_q * group / fa::kKv8ChunkRows + batch;
+    pl.chunk_blocks = (int)(most < by_rows ? most : by_rows);
+    const int64_t wgs = heads_k * pl.chunk_blocks;
     int64_t n = wgs >= 256 ? 1 : ceil_div(512, wgs);
-    const int64_t cap = ceil_div(max_keys > 0 ? max_keys : 1, 512);
+    const int64_t cap = ceil_div(max_keys, 512);
     n = n < cap ? n : cap;
-    pl.chunk_keys = (int)(ceil_div(ceil_div(max_keys > 0 ? max_keys : 1, n), 64) * 64);
-    pl.chunk_splits = (int)ceil_div(max_keys > 0 ? max_keys : 1, pl.chunk_keys);
+    pl.chunk_keys = (int)(ceil_div(ceil_div(max_keys, n), 64) * 64);
+    pl.chunk_splits = (int)ceil_div(max_keys, pl.chunk_keys);
   }
   const int most = pl.num_splits > pl.chunk_splits ? pl.num_splits : pl.chunk_splits;
   pl.workspace = most > 1 ? most * total_q * heads_q * (head_dim + 1) * 4 : 0;
@@ -214,7 +214,7 @@ extern "C" int fa_kvcache8_append(const void* k, const void* v, const int64_t* k
   return hip_status(fa_launch_kv8_append(dtype, store, p, (int)head_dim, static_cast<hipStream_t>(stream)), name);
 }
 
-extern "C" int fa_fwd_kvcache8_plan(int packed, int64_t batch, int64_t max_seqlen_q, int64_t total_q,
+extern "C" int fa_fwd_kvcache8_plan(int64_t batch, int64_t max_seqlen_q, int64_t total_q,
                                     int64_t heads_q, int64_t heads_k, int64_t head_dim, int64_t max_keys,
                                     int64_t* workspace_bytes) {
   const char* name = "fa_fwd_kvcache8_plan";
@@ -222,7 +222,7 @@ extern "C" int fa_fwd_kvcache8_plan(int packed, int64_t batch, int64_t max_seqle
   if (int st = check_plan(name, batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys); st != FA_OK)
     return st;
   *workspace_bytes =
-      make_plan(packed != 0, batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys).workspace;
+      make_plan(batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys).workspace;
   return fa_set_error(FA_OK, "");
 }
 
@@ -264,8 +264,7 @@ extern "C" int fa_fwd_kvcache8(const void* q, void* out, const int64_t* q_stride
   if (k_cache_stride[1] < head_dim || v_cache_stride[1] < head_dim || k_cache_stride[1] > kMaxSlotStride ||
       v_cache_stride[1] > kMaxSlotStride)
     return fail(FA_ERR_UNSUPPORTED, "%s: slots that overlap or lie more than 2^26 bytes apart", name);
-  const Plan pl =
-      make_plan(cu_seqlens_q != nullptr, batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys);
+  const Plan pl = make_plan(batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys);
   if (workspace_bytes < pl.workspace || (pl.workspace > 0 && workspace == nullptr))
     return fail(FA_ERR_INVALID, "%s: the workspace must be as large as fa_fwd_kvcache8_plan says", name);
   fa::Kv8AttnParams p;
@@ -304,7 +303,6 @@ extern "C" int fa_fwd_kvcache8(const void* q, void* out, const int64_t* q_stride
   p.window_right = clamp_window(window_right);
   p.split_keys = pl.split_keys;
   p.num_splits = pl.num_splits;
-  p.chunk_rows = fa::kKv8ChunkRows;
   p.chunk_blocks = pl.chunk_blocks;
   p.chunk_keys = pl.chunk_keys;
   p.chunk_splits = pl.chunk_splits;

@@ -585,7 +585,8 @@ void kv8_split_kernel(const Kv8AttnParams p) {
 }
 
 
-// kv8_chunk_kernel: more than 32 query rows per K/V head.  A workgroup of RW x
+// kv8_chunk_kernel: launches with sequences of more than 32 query rows per K/V
+// head, and the shorter ones beside them.  A workgroup of RW x
 // KG waves owns 32 RW rows, 32 per wave; its KG groups of RW waves take the
 // 64-key tiles in turn (each group with a ring of its own, whose tiles its waves
 // load together) and are merged at the end, so that a workgroup's chain of
@@ -606,22 +607,46 @@ struct Kv8Chunk {
   static constexpr int kSuper = kThreads * 16 / kBN;        // tiles whose pages and scales LDS holds
 };
 
-// The r-th sequence by descending work (queries times keys; r counted within
-// its block of 64 consecutive ones): long ones first, so that they do not start
-// last.  Every lane of the wave takes part.
-__device__ inline int kv8_nth_heaviest(const Kv8AttnParams& p, int r) {
-  const int base = r & ~63, m = min(64, p.batch - base), l = threadIdx.x & 63;
-  uint32_t key = 0;
-  if (l < m) {
-    const Kv8Rows s = kv8_rows(p, base + l);
-    // (unique: the work in 25 bits of its order of magnitude, then the earlier one)
-    const float work = (float)s.n * (float)s.L;
-    key = ((__float_as_uint(work) >> 6) & ~63u) + 64u + (uint32_t)(63 - l);
+// Row blocks of bm rows of all sequences, those of the longest chains of keys
+// first (within blocks of 64 sequences), so that a launch does not end with
+// one: the sequence of row block i and, in *rb, which of its blocks it is.
+// False past the last one.  Every lane of the wave takes part; sequences
+// without queries have none, so the host's count of them (from the rows of q)
+// bounds i without knowing the lengths.
+__device__ inline bool kv8_row_block(const Kv8AttnParams& p, int i, int bm, Kv8Rows* s, int* rb) {
+  const int l = threadIdx.x & 63, G = (int)p.group.d;
+  for (int base = 0; base < p.batch; base += 64) {
+    const int m = min(64, p.batch - base);
+    int nb = 0;
+    uint32_t key = 0;
+    Kv8Rows mine = {};
+    if (l < m) {
+      mine = kv8_rows(p, base + l);
+      nb = (mine.n * G + bm - 1) / bm;
+      // (unique: the chain in 25 bits of its float, then the earlier sequence)
+      const float chain = (float)mine.L * (float)(32 + min(mine.n * G, bm));
+      key = ((__float_as_uint(chain) >> 6) & ~63u) + 64u + (uint32_t)(63 - l);
+    }
+    int before = 0, total = 0;
+    for (int j = 0; j < m; ++j) {
+      const int nj = __builtin_amdgcn_readlane(nb, j);
+      total += nj;
+      before += (uint32_t)__builtin_amdgcn_readlane(key, j) > key ? nj : 0;
+    }
+    if (i >= total) {
+      i -= total;
+      continue;
+    }
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(i >= before && i < before + nb);
+    const int j = hit != 0 ? (int)__builtin_ctzll(hit) : 0;   // (there is one)
+    s->b = base + j;
+    s->n = __builtin_amdgcn_readlane(mine.n, j);
+    s->L = __builtin_amdgcn_readlane(mine.L, j);
+    s->q0 = (int64_t)__builtin_amdgcn_readlane((int)mine.q0, j);
+    *rb = __builtin_amdgcn_readlane(nb, j) - 1 - (i - __builtin_amdgcn_readlane(before, j));
+    return true;
   }
-  int rank = 0;
-  for (int j = 0; j < m; ++j) rank += (uint32_t)__builtin_amdgcn_readlane(key, j) > key ? 1 : 0;
-  const uint64_t hit = __builtin_amdgcn_ballot_w64(l < m && rank == (r & 63));
-  return base + (hit != 0 ? (int)__builtin_ctzll(hit) : 0);
+  return false;
 }
 
 template <class T, class F8, int D, int RW, int KG, int NST, bool GENERIC>
@@ -641,30 +666,17 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
   const int rw = w % RW, kg = w / RW;
   const int c32 = lane & 31, g = lane >> 5;
 
-  // Work item: the K/V heads of the sequences, heaviest sequence first, are
-  // dealt round over the XCDs, all row blocks (and splits) of one on the same, so
-  // that they share its keys in the L2; the last ones, too few for a round, are
-  // spread over all.
-  const int per = p.chunk_blocks * p.chunk_splits;
-  const int main = p.batch * p.heads_k / 8 * 8;
-  int item = blockIdx.x, c, i;
-  if (item < main * per) {
-    const int k = item / 8;
-    c = k / per * 8 + item % 8;
-    i = k % per;
-  } else {
-    item -= main * per;
-    c = main + item / per;
-    i = item % per;
-  }
-  const int b = kv8_nth_heaviest(p, c / p.heads_k);
-  const int kvh = c % p.heads_k;
-  const int rb = p.chunk_blocks - 1 - i / p.chunk_splits, split = i % p.chunk_splits;
-
-  const Kv8Rows s = kv8_rows(p, b);
-  const int G = (int)p.group.d;
+  // K/V heads vary fastest: with 8 of them, or a multiple, each XCD streams its
+  // own heads' keys, and all XCDs get the same work.
+  int item = blockIdx.x;
+  const int kvh = item % p.heads_k;
+  item /= p.heads_k;
+  const int split = item % p.chunk_splits;
+  Kv8Rows s;
+  int rb;
+  if (!kv8_row_block(p, item / p.chunk_splits, BM, &s, &rb)) return;
+  const int b = s.b, G = (int)p.group.d;
   const int rows = min(s.n * G - rb * BM, BM);
-  if (rows <= 0 || s.n * G <= kKv8SplitRows) return;
   int lo, hi;
   kv8_key_range(p, s, (int)fdiv(rb * BM, p.group), (int)fdiv(rb * BM + rows - 1, p.group), lo, hi);
   const int k_begin = max(split * p.chunk_keys, lo & ~(BN - 1));
@@ -883,26 +895,18 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
   }
 }
 
-// Merges the splits of each row: out = sum_s 2^(lse_s - lse) o_s over the
-// splits that hold keys its workgroup saw (the others are unwritten).  One
-// thread per row and 4 dims, a workgroup within one sequence; partials are
-// fetched in batches of independent loads.
+// Merges the splits of four dims of a row: out = sum_s 2^(lse_s - lse) o_s over
+// the splits that hold keys its workgroup saw (the others are unwritten), the
+// partials fetched in batches of independent loads.  item: query * heads + head.
 template <class T, int D>
-__global__ __launch_bounds__(256) void kv8_combine_kernel(const Kv8AttnParams p) {
+__device__ inline void kv8_combine_row(const Kv8AttnParams& p, const Kv8Rows& s, int64_t item, int qd) {
   constexpr int kBatch = 8;
-  constexpr int kQuads = D / 4;
-  const int b = blockIdx.y;
-  const Kv8Rows s = kv8_rows(p, b);
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t item = idx / kQuads;
-  if (item >= (int64_t)s.n * p.heads_q) return;
-  const int qd = (int)(idx % kQuads), h = (int)(item % p.heads_q), i = (int)(item / p.heads_q);
+  const int h = (int)(item % p.heads_q), i = (int)(item / p.heads_q);
   const int G = (int)p.group.d;
   // The splits that the row's workgroups ran: those that meet their keys.
-  const bool chunk = s.n * G > kKv8SplitRows;
+  const bool chunk = p.chunk_splits > 0;
   const int splits = chunk ? p.chunk_splits : p.num_splits, keys = chunk ? p.chunk_keys : p.split_keys;
-  if (splits == 1) return;   // (written by the row's only workgroup)
-  const int bm = chunk ? p.chunk_rows : kKv8SplitRows;
+  const int bm = chunk ? kKv8ChunkRows : kKv8SplitRows;
   const int rb = (i * G + h % G) / bm, last = min(rb * bm + bm - 1, s.n * G - 1);
   int lo, hi;
   kv8_key_range(p, s, (int)fdiv(rb * bm, p.group), (int)fdiv(last, p.group), lo, hi);
@@ -949,6 +953,16 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(const Kv8AttnParams p)
   *reinterpret_cast<u32x2*>(dst) = val;
 }
 
+// One thread per row and 4 dims, a workgroup within one sequence.
+template <class T, int D>
+__global__ __launch_bounds__(256) void kv8_combine_kernel(const Kv8AttnParams p) {
+  constexpr int kQuads = D / 4;
+  const Kv8Rows s = kv8_rows(p, blockIdx.y);
+  for (int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; idx < (int64_t)s.n * p.heads_q * kQuads;
+       idx += (int64_t)gridDim.x * 256)
+    kv8_combine_row<T, D>(p, s, idx / kQuads, (int)(idx % kQuads));
+}
+
 template <class T, class F8, int D, bool GENERIC>
 hipError_t launch_kv8(const Kv8AttnParams& p, hipStream_t st) {
   if (p.num_splits > 0) {
@@ -969,14 +983,16 @@ hipError_t launch_kv8(const Kv8AttnParams& p, hipStream_t st) {
     auto kern = kv8_chunk_kernel<T, F8, D, RW, KG, NST, GENERIC>;
     static std::atomic<uint64_t> lds_devices{0};
     if (hipError_t e = set_lds_limit(lds_devices, kern, C::kLds); e != hipSuccess) return e;
-    const int64_t wgs = (int64_t)p.chunk_splits * p.chunk_blocks * p.batch * p.heads_k;
+    const int64_t wgs = (int64_t)p.chunk_splits * p.chunk_blocks * p.heads_k;
     if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(C::kThreads), C::kLds, st, p);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   if (p.num_splits <= 1 && p.chunk_splits <= 1) return hipSuccess;
-  const int64_t threads = (int64_t)p.seqlen_q * p.heads_q * (D / 4);
-  hipLaunchKernelGGL((kv8_combine_kernel<T, D>), dim3((unsigned)((threads + 255) / 256), (unsigned)p.batch),
+  // (few workgroups per sequence: most sequences of a packed batch are far
+  // shorter than its longest)
+  const int64_t wgs = ((int64_t)p.seqlen_q * p.heads_q * (D / 4) + 255) / 256, cap = 8192 / p.batch + 1;
+  hipLaunchKernelGGL((kv8_combine_kernel<T, D>), dim3((unsigned)(wgs < cap ? wgs : cap), (unsigned)p.batch),
                      dim3(256), 0, st, p);
   return hipGetLastError();
 }

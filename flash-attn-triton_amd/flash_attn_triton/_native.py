@@ -92,7 +92,7 @@ _SIGNATURES = {
                                 _vp, _vp, _vp, _vp]),
     "fa_kvcache8_append": (_int, [_vp, _vp, _i64p, _i64p, _int, _vp, _vp, _i64p, _i64p, _int, _vp, _vp,
                                   _i64p, _i64p, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
-    "fa_fwd_kvcache8_plan": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64p]),
+    "fa_fwd_kvcache8_plan": (_int, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64p]),
     "fa_fwd_kvcache8": (_int, [_vp, _vp, _i64p, _i64p, _int, _vp, _vp, _i64p, _i64p, _int, _vp, _vp,
                                _i64p, _i64p, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64,
                                _i64, _i64, _i64, _i64, _i64, _f32, _int, _i64, _i64, _f32, _vp, _i64,
@@ -498,11 +498,11 @@ def kvcache8_append(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapping) -> N
 
 
 @functools.lru_cache(maxsize=1024)
-def kvcache8_plan(packed: bool, batch: int, max_seqlen_q: int, total_q: int, heads_q: int, heads_k: int,
-                  head_dim: int, max_keys: int) -> int:
+def kvcache8_plan(batch: int, max_seqlen_q: int, total_q: int, heads_q: int, heads_k: int, head_dim: int,
+                  max_keys: int) -> int:
     """Workspace bytes of fwd_kvcache8."""
     ws = ctypes.c_int64(0)
-    _check(load().fa_fwd_kvcache8_plan(packed, batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys,
+    _check(load().fa_fwd_kvcache8_plan(batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys,
                                        ctypes.byref(ws)), "fa_fwd_kvcache8_plan")
     return int(ws.value)
 
@@ -516,7 +516,7 @@ def fwd_kvcache8(q, out, k_cache, v_cache, k_scale, v_scale, cache_seqlens, bloc
     pages, page, Hk = k_cache.shape[:3]
     packed = cu_seqlens_q is not None
     total = q.shape[0] if packed else batch * max_seqlen_q
-    ws_bytes = kvcache8_plan(packed, batch, max_seqlen_q, total, Hq, Hk, D, max_keys)
+    ws_bytes = kvcache8_plan(batch, max_seqlen_q, total, Hq, Hk, D, max_keys)
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     qs, os_ = q.stride(), out.stride()
     q_stride = _strides((0,) + qs[:2] if packed else qs[:3])

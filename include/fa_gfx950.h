@@ -470,9 +470,9 @@ int fa_kvcache8_append(const void* k, const void* v, const int64_t* k_stride, co
                        fa_stream_t stream);
 
 /* Bytes of workspace (fp32 partial rows of the key splits) of fa_fwd_kvcache8
- * for these sizes; packed: with cu_seqlens_q.  Host only. */
-int fa_fwd_kvcache8_plan(int packed, int64_t batch, int64_t max_seqlen_q, int64_t total_q,
-                         int64_t heads_q, int64_t heads_k, int64_t head_dim, int64_t max_keys,
+ * for these sizes.  Host only. */
+int fa_fwd_kvcache8_plan(int64_t batch, int64_t max_seqlen_q, int64_t total_q, int64_t heads_q,
+                         int64_t heads_k, int64_t head_dim, int64_t max_keys,
                          int64_t* workspace_bytes);
 
 /* Attention of queries against the 8-bit cache: fa_fwd_kvcache with q and out

@@ -110,7 +110,7 @@ def test_c_attention_checks(lib):
     def call(q=one, dtype=0, store=0, table=one, cols=4, pages=8, page=32, block=16, cu=None, batch=2, max_q=1, total=2,
              max_keys=128, hq=2, hk=1, dim=64, less=0, ws=one, kst=st, softcap=0.0):
         need = ctypes.c_int64(0)
-        lib.fa_fwd_kvcache8_plan(0, batch, max_q, total, hq, hk, dim, max_keys, ctypes.byref(need))
+        lib.fa_fwd_kvcache8_plan(batch, max_q, total, hq, hk, dim, max_keys, ctypes.byref(need))
         return lib.fa_fwd_kvcache8(q, one, st, st, dtype, one, one, kst, kst, store, one, one, st, st, one, table, 4, cols,
                                    pages, page, block, cu, batch, max_q, total, max_keys, hq, hk, dim, 1.0, 1, -1, -1,
                                    softcap, None, 0, ws, need.value - less, None)
@@ -131,10 +131,10 @@ def test_c_attention_checks(lib):
 
 def test_plan_asks_for_whole_rows(lib):
     # fp32 rows and a sum for every split of every row of q
-    for args in ((0, 1, 1, 1, 32, 8, 128, 131001), (0, 64, 1, 64, 32, 8, 128, 8192), (1, 3, 700, 900, 16, 4, 64, 4000)):
+    for args in ((1, 1, 1, 32, 8, 128, 131001), (64, 1, 64, 32, 8, 128, 8192), (3, 40, 50, 16, 4, 64, 4000)):
         need = ctypes.c_int64(0)
         assert lib.fa_fwd_kvcache8_plan(*args, ctypes.byref(need)) == _native.FA_OK
-        assert need.value > 0 and need.value % (args[3] * args[4] * (args[6] + 1) * 4) == 0
+        assert need.value > 0 and need.value % (args[2] * args[3] * (args[5] + 1) * 4) == 0
 
 
 def test_scale_rule():
