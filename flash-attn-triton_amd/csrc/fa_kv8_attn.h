@@ -256,18 +256,22 @@ __device__ inline void kv8_exp(const f32x16& sc, float sl, float m, u32x4* pb, f
     }
 }
 
-// O^T += V^T P^T over the 32 keys of V in LDS from row0 on, scaled by vsc (16
-// keys each).  mixed: the rows of the wave do not all see all of these keys, and
-// a V number that is not finite must not meet a P of 0.
-template <class T, class F8, int D>
-__device__ inline void kv8_pv(const uint8_t* vt, const Kv8Lane<D>& at, int row0, const float* vsc,
-                              const u32x4* pb, const f32x16& sc, bool mixed, f32x16* acc) {
-  constexpr int NDB = D / 32;
-  u32x2 raw[2][NDB];
+// The V^T operand of 32 keys of a tile in LDS, from row0 on: 8 bytes per 16-key
+// step and 32 dims.  Read before the scores are turned into probabilities.
+template <int D>
+__device__ inline void kv8_read_v(const uint8_t* vt, const Kv8Lane<D>& at, int row0, u32x2 (*raw)[D / 32]) {
 #pragma unroll
   for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
-    for (int db = 0; db < NDB; ++db) raw[cc][db] = lds_read_tr8(vt + at.v[db] + (row0 + 16 * cc) * D);
+    for (int db = 0; db < D / 32; ++db) raw[cc][db] = lds_read_tr8(vt + at.v[db] + (row0 + 16 * cc) * D);
+}
+
+// O^T += V^T P^T over 32 keys, V scaled by vsc (16 keys each).  mixed: the rows of the wave do not all see all of these keys, and
+// a V number that is not finite must not meet a P of 0.
+template <class T, class F8, int D>
+__device__ inline void kv8_pv(u32x2 (*raw)[D / 32], const float* vsc, const u32x4* pb, const f32x16& sc,
+                              bool mixed, f32x16* acc) {
+  constexpr int NDB = D / 32;
   if (mixed) {
     uint32_t flags = 0;
 #pragma unroll
@@ -314,6 +318,38 @@ __device__ inline void kv8_pv(const uint8_t* vt, const Kv8Lane<D>& at, int row0,
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
       acc[db] = T::mfma32(kv8_operand<T, F8>(raw[cc][db][0], raw[cc][db][1], vsc[cc]), pb[cc], acc[db]);
+}
+
+// Steps 0 .. n - 1 in order, those in [b, e) by step(i, false_type), the others
+// by step(i, true_type).  Loops of their own: one loop with both forms would
+// copy the accumulators where they join, and a mask between the products and
+// the maximum, in a block of its own, costs an instruction per score there.
+template <class F>
+__device__ inline void kv8_three_runs(int n, int b, int e, F step) {
+  int i = 0, upto = b < e ? b : n;
+  while (true) {
+    for (; i < upto; ++i) step(i, std::true_type{});
+    if (i >= n) break;
+    for (; i < e; ++i) step(i, std::false_type{});
+    upto = n;
+    if (i >= n) break;
+  }
+}
+__device__ inline int kv8_clamp(int x, int n) { return x < 0 ? 0 : x > n ? n : x; }
+// The first i >= 0 with i * per >= x.
+__device__ inline int ceil_steps(int x, int per) { return x <= 0 ? 0 : (x + per - 1) / per; }
+
+// Largest of a lane's NH x 16 scores, in four chains of v_max3.
+template <int NH>
+__device__ inline float kv8_max(const f32x16* sc) {
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int h = 0; h < NH; ++h)
+#pragma unroll
+    for (int v = 0; v < 16; v += 8)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) m[q] = fmaxf(fmaxf(m[q], sc[h][v + 2 * q]), sc[h][v + 2 * q + 1]);
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
 // Raises the running maximum m (log2 units) of rows whose new one passes it by
@@ -473,7 +509,7 @@ void kv8_split_kernel(const Kv8AttnParams p) {
   for (int j = 0; j < 2 * NDB; ++j) asm volatile("" : "+v"(qreg[j]));
   asm volatile("" : "+v"(ks_l), "+v"(vs_l));
   if (GENERIC) asm volatile("" : "+v"(row.slope));
-  for (int t = 0; t < my_tiles; ++t) {
+  auto step = [&](int t, auto masked) {
     const int n0 = k_begin + (w + t * kKv8Waves) * BN;
     // (this wave's LDS reads of the stage that is filled now ended with the
     // previous tile's products)
@@ -482,31 +518,29 @@ void kv8_split_kernel(const Kv8AttnParams p) {
     __builtin_amdgcn_s_waitcnt(vmcnt_imm((NST - 1) * 2 * NI + NI));   // K of tile t
     asm volatile("" ::: "memory");
     const uint8_t* kt = ring + (t % NST) * 2 * Tile::kBytes;
-    const uint8_t* vt = kt + Tile::kBytes;
-
     const float ks0 = __uint_as_float(__builtin_amdgcn_readlane(ks_l, 2 * t));
     const float ks1 = __uint_as_float(__builtin_amdgcn_readlane(ks_l, 2 * t + 1));
     const float ksc = c32 < 16 ? ks0 : ks1;
     f32x16 sc;
     kv8_qk<T, F8, D, 1>(kt, at, &ksc, qreg, &sc);
     if (GENERIC) kv8_score_options(p, row, n0, sc);
-    if (n0 < all_lo || n0 + BN - 1 > all_hi) kv8_mask(row, n0, sc);
-    float mx = -INFINITY;
-#pragma unroll
-    for (int v = 0; v < 16; v += 2) mx = fmaxf(mx, fmaxf(sc[v], sc[v + 1]));
-    mx = halves_max(mx) * sl;
-    kv8_raise<NDB>(mx, m_run, l_run, acc);
+    if (masked.value) kv8_mask(row, n0, sc);
+    kv8_raise<NDB>(halves_max(kv8_max<1>(&sc)) * sl, m_run, l_run, acc);
     u32x4 pb[2];
     kv8_exp<T>(sc, sl, m_run == -INFINITY ? 0.f : m_run, pb, l_run);
-
     __builtin_amdgcn_s_waitcnt(vmcnt_imm((NST - 1) * 2 * NI));   // V of tile t
     asm volatile("" ::: "memory");
     const float vsc[2] = {__uint_as_float(__builtin_amdgcn_readlane(vs_l, 2 * t)),
                           __uint_as_float(__builtin_amdgcn_readlane(vs_l, 2 * t + 1))};
+    u32x2 raw[2][NDB];
+    kv8_read_v<D>(kt + Tile::kBytes, at, 0, raw);
     // (keys past the sequence's end are zeros in V)
-    const bool mixed = n0 < all_lo || (n0 + BN - 1 > all_hi && all_hi < s.L - 1);
-    kv8_pv<T, F8, D>(vt, at, 0, vsc, pb, sc, mixed, acc);
-  }
+    const bool mixed = masked.value && (n0 < all_lo || (n0 + BN - 1 > all_hi && all_hi < s.L - 1));
+    kv8_pv<T, F8, D>(raw, vsc, pb, sc, mixed, acc);
+  };
+  const int first = k_begin + w * BN;
+  kv8_three_runs(my_tiles, kv8_clamp(ceil_steps(all_lo - first, kKv8Waves * BN), my_tiles),
+                 kv8_clamp(ceil_steps(all_hi + 1 - BN + 1 - first, kKv8Waves * BN), my_tiles), step);
 
   // ------------------------------------------------------------ merge waves
   // The rings become the rows' merge area once every load into them has landed
@@ -755,9 +789,9 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
     __syncthreads();
 
     // This wave's share of tile kg + KG * step into its stage.
-    auto issue = [&](int step) {
+    auto issue = [&](int step, uint32_t stage) {
       const int t = kg + KG * step;
-      const uint32_t st = ring_lds + (uint32_t)((step % NST) * 2 * C::kTile);
+      const uint32_t st = ring_lds + stage;
       const int row_l = lane / CPR, pos = lane % CPR;
 #pragma unroll
       for (int u = 0; u < GPW; ++u) {
@@ -784,48 +818,56 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
       }
     };
 
-    for (int i0 = 0; i0 < NST - 1; ++i0) issue(i0);
+    for (int i0 = 0; i0 < NST - 1; ++i0) issue(i0, (uint32_t)(i0 * 2 * C::kTile));
 #pragma unroll
     for (int j = 0; j < 2 * NDB; ++j) asm volatile("" : "+v"(qreg[j]));
     if (GENERIC) asm volatile("" : "+v"(row.slope));
-    for (int i0 = 0; i0 < steps; ++i0) {
-      // Tile i0 has landed, for every wave, and the stage that is filled next
+    uint32_t stage = 0, next_stage = (uint32_t)((NST - 1) * 2 * C::kTile);   // of tiles i0 and i0 + NST - 1
+    auto advance = [](uint32_t st) { return st + 2 * C::kTile == NST * 2 * C::kTile ? 0u : st + 2 * C::kTile; };
+    // Step i: every wave passes its barrier, whatever it does with the tile.
+    auto step = [&](int i, auto masked) {
+      // Tile i has landed, for every wave, and the stage that is filled next
       // has been read.
       __builtin_amdgcn_sched_barrier(0);
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NST - 2) * PER) : "memory");
       __builtin_amdgcn_sched_barrier(0);
-      issue(i0 + NST - 1);
-      const int t = kg + KG * i0;
-      const int n0 = s0 + t * BN;
-      if (t >= n_tiles || n0 >= whi || n0 + BN <= wlo) continue;
-      const uint8_t* kt = ring + (i0 % NST) * 2 * C::kTile;
+      issue(i + NST - 1, next_stage);
+      const int t = kg + KG * i, n0 = s0 + t * BN;
+      const uint8_t* kt = ring + stage;
       const uint8_t* vt = kt + C::kTile;
-      const bool masked = n0 < all_lo || n0 + BN - 1 > all_hi || n0 + BN > k_end;
-      f32x16 sc[2];
-      float mx = -INFINITY;
+      stage = advance(stage);
+      next_stage = advance(next_stage);
+      if (masked.value && (t >= n_tiles || n0 >= whi || n0 + BN <= wlo)) return;
       const float ksc[2] = {__uint_as_float((info_scale[4 * t + (c32 >> 4)] & 0xffffu) << 23),
                             __uint_as_float((info_scale[4 * t + 2 + (c32 >> 4)] & 0xffffu) << 23)};
+      float vsc[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) vsc[u] = __uint_as_float(info_scale[4 * t + u] >> 16 << 23);
+      f32x16 sc[2];
       kv8_qk<T, F8, D, 2>(kt, at, ksc, qreg, sc);
+      u32x2 raw[2][2][NDB];
+      kv8_read_v<D>(vt, at, 0, raw[0]);
+      kv8_read_v<D>(vt, at, 32, raw[1]);
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         if (GENERIC) kv8_score_options(p, row, n0 + 32 * hf, sc[hf]);
-        if (masked) kv8_mask(row, n0 + 32 * hf, sc[hf]);
-#pragma unroll
-        for (int v = 0; v < 16; v += 2) mx = fmaxf(mx, fmaxf(sc[hf][v], sc[hf][v + 1]));
+        if (masked.value) kv8_mask(row, n0 + 32 * hf, sc[hf]);
       }
-      mx = halves_max(mx) * sl;
-      kv8_raise<NDB>(mx, m_run, l_run, acc);
+      kv8_raise<NDB>(halves_max(kv8_max<2>(sc)) * sl, m_run, l_run, acc);
       const float m_use = m_run == -INFINITY ? 0.f : m_run;
-      const bool mixed = n0 < all_lo || (n0 + BN - 1 > all_hi && all_hi < s.L - 1);
+      const bool mixed = masked.value && (n0 < all_lo || (n0 + BN - 1 > all_hi && all_hi < s.L - 1));
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         u32x4 pb[2];
         kv8_exp<T>(sc[hf], sl, m_use, pb, l_run);
-        const float vsc[2] = {__uint_as_float(info_scale[4 * t + 2 * hf] >> 16 << 23),
-                              __uint_as_float(info_scale[4 * t + 2 * hf + 1] >> 16 << 23)};
-        kv8_pv<T, F8, D>(vt, at, 32 * hf, vsc, pb, sc[hf], mixed, acc);
+        kv8_pv<T, F8, D>(raw[hf], vsc + 2 * hf, pb, sc[hf], mixed, acc);
       }
-    }
+    };
+    // Steps [i_b, i_e) of this wave need no mask.
+    const int first = s0 + kg * BN;
+    const int i_b = kv8_clamp(ceil_steps(all_lo - first, KG * BN), steps);
+    const int i_e = wrows > 0 ? kv8_clamp(ceil_steps(min(all_hi + 1, k_end) - BN + 1 - first, KG * BN), steps) : 0;
+    kv8_three_runs(steps, i_b, i_e, step);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
 
