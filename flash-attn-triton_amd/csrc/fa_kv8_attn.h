@@ -46,6 +46,7 @@ static_assert(kKv8MaxSplit == 32 * kKv8Waves * kKv8BN, "64 lanes hold the 16-key
 // The 8-bit types.  bad(): the high bit of each byte of a word whose number is
 // not finite.
 struct E4M3 {
+  static constexpr int kFormat = 0;   // of the scaled MFMA
   template <class T>
   __device__ static inline uint32_t cvt(uint32_t w, float scale, bool hi);
   __device__ static inline uint32_t bad(uint32_t w) {
@@ -53,6 +54,7 @@ struct E4M3 {
   }
 };
 struct E5M2 {
+  static constexpr int kFormat = 1;
   template <class T>
   __device__ static inline uint32_t cvt(uint32_t w, float scale, bool hi);
   __device__ static inline uint32_t bad(uint32_t w) {
@@ -176,9 +178,9 @@ __device__ inline Kv8Row kv8_row(const Kv8AttnParams& p, const Kv8Rows& s, int q
 
 // Byte offsets of a lane's operand reads in a tile of 32 keys (the swizzles
 // repeat every 16 rows, so the other steps and halves are constants away).  K:
-// row lane % 32, chunk 2 j + lane / 32.  V: the lane's 8 keys of 16-key step cc
+// row lane % 32, the chunks of Kv8Query.  V: the lane's 8 keys of 16-key step cc
 // are 16 cc + 4 g + {0..3, 8..11}; lane i of 16 names 8 bytes of row i / 2.
-template <int D>
+template <int D, class Q>
 struct Kv8Lane {
   uint32_t k[D / 32], v[D / 32];
   __device__ inline Kv8Lane() {
@@ -186,34 +188,133 @@ struct Kv8Lane {
     const int vr = (lane & 15) >> 1, vkey = 4 * g + (vr & 3) + 8 * (vr >> 2);
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
-      k[j] = (uint32_t)(c32 * D + kv8_k_chunk<D>(c32, 2 * j + g) * 16);
+      k[j] = (uint32_t)(c32 * D + kv8_k_chunk<D>(c32, Q::chunk(j, g)) * 16);
       v[j] = (uint32_t)(vkey * D + kv8_v_chunk<D>(vkey, 2 * j + ((lane >> 4) & 1)) * 16 + 8 * (lane & 1));
     }
   }
 };
 
-// S^T of NH x 32 keys: the rows of a K tile in LDS against Q^T in registers,
-// each row scaled by its key's ksc[h].  Every operand is read before the first
-// product, and the products of the halves take turns: neither an LDS read nor
-// the chain of one accumulator is waited for in between.
-template <class T, class F8, int D, int NH>
-__device__ inline void kv8_qk(const uint8_t* kt, const Kv8Lane<D>& at, const float* ksc, const u32x4* qreg,
-                              f32x16* sc) {
-  u32x4 raw[NH][D / 32];
+// The queries of a wave as the B operand of S^T = K Q^T, and the product.
+//
+// fp16: 16-bit products.  K rows become 16-bit operands: 4 conversions per
+// product.  A lane's chunk j of a row is dims 32 j + 16 g .., its low 8 for
+// product 2 j and the high 8 for product 2 j + 1.
+template <class T, int D>
+struct Kv8Query {
+  u32x4 q[D / 16];
+  __device__ static inline int chunk(int j, int g) { return 2 * j + g; }
+  __device__ inline void load(const uint16_t* row) {
+    const int g = (threadIdx.x >> 5) & 1;
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j)
+    for (int j = 0; j < D / 32; ++j) {
+      q[2 * j] = load16(row + 32 * j + 16 * g);
+      q[2 * j + 1] = load16(row + 32 * j + 16 * g + 8);
+    }
+  }
+  // Waits for the loads (see the call).
+  __device__ inline void pin() {
 #pragma unroll
-    for (int h = 0; h < NH; ++h) raw[h][j] = load16(kt + at.k[j] + 32 * h * D);
+    for (int j = 0; j < D / 16; ++j) asm volatile("" : "+v"(q[j]));
+  }
+  // S^T of NH x 32 keys: the rows of a K tile in LDS, each scaled by its key's
+  // scale byte.  The products of the halves take turns, so that the chain of one
+  // accumulator is not waited for.
+  template <class F8, int NH, class Lane>
+  __device__ inline void scores(const uint8_t* kt, const Lane& at, const uint32_t* byte, f32x16* sc) const {
+    u32x4 raw[NH][D / 32];
 #pragma unroll
-  for (int h = 0; h < NH; ++h) sc[h] = f32x16{};
+    for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j)
+      for (int h = 0; h < NH; ++h) raw[h][j] = load16(kt + at.k[j] + 32 * h * D);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int h = 0; h < NH; ++h) sc[h] = f32x16{};
 #pragma unroll
-      for (int h = 0; h < NH; ++h)
-        sc[h] = T::mfma32(kv8_operand<T, F8>(raw[h][j][2 * u], raw[h][j][2 * u + 1], ksc[h]), qreg[2 * j + u], sc[h]);
-}
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+          sc[h] = T::mfma32(kv8_operand<T, F8>(raw[h][j][2 * u], raw[h][j][2 * u + 1],
+                                               __uint_as_float(byte[h] << 23)),
+                            q[2 * j + u], sc[h]);
+  }
+};
+
+// bf16: 8-bit products (v_mfma_scale_f32_32x32x64), which take K as it is and
+// its scale with it.  A bf16 number has 8 significant bits and e4m3 holds 4, so
+// the query is the sum of two 8-bit ones, q = 2^e (q1 + q2 / 16), exactly as
+// far as the type's range goes: to 2^-23 of the row's largest number, below
+// what the fp32 sums of the products are off by.  Two products at twice the
+// rate take the time of one in 16 bits, and the 4 conversions per product go.
+// (fp16 has 11 bits: three products.)  chunk(j): the 16-byte halves of dims
+// 64 (j / 2) + 32 g ...
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+template <int D>
+struct Kv8Query<BF16, D> {
+  i32x8 q[2][D / 64];
+  int byte;   // e + 127
+  __device__ static inline int chunk(int j, int g) { return 4 * (j / 2) + 2 * g + (j & 1); }
+  u32x4 raw_[D / 16];
+  __device__ inline void load(const uint16_t* row) {
+    const int g = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) raw_[j] = load16(row + 64 * (j / 4) + 32 * g + 8 * (j % 4));
+  }
+  __device__ inline void pin() {
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) asm volatile("" : "+v"(raw_[j]));
+    uint32_t top = 0;   // largest magnitude, as the bits of a bf16
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, max(raw_[j][e] & 0x7fffu, (raw_[j][e] >> 16) & 0x7fffu));
+    auto r = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+    top = max((uint32_t)r[0], (uint32_t)r[1]);
+    // The least e with top <= 1.75 * 2^(8 + e); NaN and infinities: a NaN scale.
+    byte = (int)(top >> 7) - 8 + ((top & 0x7fu) > 0x60u ? 1 : 0);
+    byte = top >= 0x7f80u ? 255 : max(byte, 5);   // (the second part's is 4 less)
+    const float by = __uint_as_float((uint32_t)(254 - min(byte, 253)) << 23);
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {   // four numbers
+      float x[4], y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[e] = BF16::to_float((uint16_t)(raw_[j / 2][2 * (j & 1) + e / 2] >> (16 * (e & 1)))) * by;
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+      y[0] = (x[0] - lo[0]) * 16.f, y[1] = (x[1] - lo[1]) * 16.f;
+      y[2] = (x[2] - hi[0]) * 16.f, y[3] = (x[3] - hi[1]) * 16.f;
+      int w2 = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      w2 = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w2, true);
+      q[0][j / 8][j % 8] = w;
+      q[1][j / 8][j % 8] = w2;
+    }
+  }
+  template <class F8, int NH, class Lane>
+  __device__ inline void scores(const uint8_t* kt, const Lane& at, const uint32_t* kbyte, f32x16* sc) const {
+    u32x4 raw[NH][D / 32];
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int h = 0; h < NH; ++h) raw[h][j] = load16(kt + at.k[j] + 32 * h * D);
+#pragma unroll
+    for (int h = 0; h < NH; ++h) sc[h] = f32x16{};
+    const int byte2 = byte == 255 ? 255 : byte - 4;
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          i32x8 a;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a[e] = (int)raw[h][2 * j + e / 4][e % 4];
+          sc[h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[u][j], sc[h], F8::kFormat, 0, 0,
+                                                                  (int)kbyte[h], 0, u ? byte2 : byte);
+        }
+  }
+};
 
 // Scale, ALiBi and softcap of the scores of keys n0 .. n0 + 31.
 __device__ inline void kv8_score_options(const Kv8AttnParams& p, const Kv8Row& row, int n0, f32x16& sc) {
@@ -258,8 +359,8 @@ __device__ inline void kv8_exp(const f32x16& sc, float sl, float m, u32x4* pb, f
 
 // The V^T operand of 32 keys of a tile in LDS, from row0 on: 8 bytes per 16-key
 // step and 32 dims.  Read before the scores are turned into probabilities.
-template <int D>
-__device__ inline void kv8_read_v(const uint8_t* vt, const Kv8Lane<D>& at, int row0, u32x2 (*raw)[D / 32]) {
+template <int D, class Lane>
+__device__ inline void kv8_read_v(const uint8_t* vt, const Lane& at, int row0, u32x2 (*raw)[D / 32]) {
 #pragma unroll
   for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
@@ -427,23 +528,16 @@ void kv8_split_kernel(const Kv8AttnParams p) {
   if (p.window_right >= 0) all_hi = min(all_hi, off + p.window_right);
   if (p.window_left >= 0) all_lo = max(0, s.n - 1 + off - p.window_left);
   // Q^T in the order of the K operand.
-  u32x4 qreg[2 * NDB];
-  {
-    const uint16_t* qrow = static_cast<const uint16_t*>(p.q) + kv8_base(p, s, p.q_sb, p.q_ss) +
-                           (int64_t)qi * p.q_ss + (int64_t)head * p.q_sh;
-#pragma unroll
-    for (int j = 0; j < NDB; ++j) {
-      qreg[2 * j] = load16(qrow + 32 * j + 16 * g);
-      qreg[2 * j + 1] = load16(qrow + 32 * j + 16 * g + 8);
-    }
-  }
+  Kv8Query<T, D> query;
+  query.load(static_cast<const uint16_t*>(p.q) + kv8_base(p, s, p.q_sb, p.q_ss) + (int64_t)qi * p.q_ss +
+             (int64_t)head * p.q_sh);
 
   // Lane i holds page, slot and scales of 16-key group i % 2 of this wave's tile
   // i / 2.  A group without keys names no page; its scale is 1.
   const int n_tiles = k_end > k_begin ? (k_end - k_begin + BN - 1) / BN : 0;
   const int my_tiles = (n_tiles - w + kKv8Waves - 1) / kKv8Waves;
   int page_l = -1, slot_l = 0;
-  uint32_t ks_l = 127u << 23, vs_l = 127u << 23;
+  uint32_t ks_l = 127, vs_l = 127;   // scale bytes
   {
     const int key = k_begin + (w + (lane >> 1) * kKv8Waves) * BN + (lane & 1) * 16;
     if (key < k_end) {
@@ -454,8 +548,8 @@ void kv8_split_kernel(const Kv8AttnParams p) {
         page_l = -1;
       } else {
         const int blk = slot_l >> p.log2_block;
-        ks_l = (uint32_t)p.ks[page_l * p.ks_sp + blk * p.ks_sb + kvh * p.ks_sh] << 23;
-        vs_l = (uint32_t)p.vs[page_l * p.vs_sp + blk * p.vs_sb + kvh * p.vs_sh] << 23;
+        ks_l = p.ks[page_l * p.ks_sp + blk * p.ks_sb + kvh * p.ks_sh];
+        vs_l = p.vs[page_l * p.vs_sp + blk * p.vs_sb + kvh * p.vs_sh];
       }
     }
   }
@@ -494,7 +588,7 @@ void kv8_split_kernel(const Kv8AttnParams p) {
     }
   };
 
-  const Kv8Lane<D> at;
+  const Kv8Lane<D, Kv8Query<T, D>> at;
   f32x16 acc[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) acc[db] = f32x16{};
@@ -505,8 +599,7 @@ void kv8_split_kernel(const Kv8AttnParams p) {
   // The compiler does not count the LDS-DMA loads: a use of a loaded register
   // inside the loop would wait there for everything in flight, so all of them
   // are waited for here, once.
-#pragma unroll
-  for (int j = 0; j < 2 * NDB; ++j) asm volatile("" : "+v"(qreg[j]));
+  query.pin();
   asm volatile("" : "+v"(ks_l), "+v"(vs_l));
   if (GENERIC) asm volatile("" : "+v"(row.slope));
   auto step = [&](int t, auto masked) {
@@ -518,11 +611,10 @@ void kv8_split_kernel(const Kv8AttnParams p) {
     __builtin_amdgcn_s_waitcnt(vmcnt_imm((NST - 1) * 2 * NI + NI));   // K of tile t
     asm volatile("" ::: "memory");
     const uint8_t* kt = ring + (t % NST) * 2 * Tile::kBytes;
-    const float ks0 = __uint_as_float(__builtin_amdgcn_readlane(ks_l, 2 * t));
-    const float ks1 = __uint_as_float(__builtin_amdgcn_readlane(ks_l, 2 * t + 1));
-    const float ksc = c32 < 16 ? ks0 : ks1;
+    const uint32_t ks0 = __builtin_amdgcn_readlane(ks_l, 2 * t), ks1 = __builtin_amdgcn_readlane(ks_l, 2 * t + 1);
+    const uint32_t ksc = c32 < 16 ? ks0 : ks1;
     f32x16 sc;
-    kv8_qk<T, F8, D, 1>(kt, at, &ksc, qreg, &sc);
+    query.template scores<F8, 1>(kt, at, &ksc, &sc);
     if (GENERIC) kv8_score_options(p, row, n0, sc);
     if (masked.value) kv8_mask(row, n0, sc);
     kv8_raise<NDB>(halves_max(kv8_max<1>(&sc)) * sl, m_run, l_run, acc);
@@ -530,8 +622,8 @@ void kv8_split_kernel(const Kv8AttnParams p) {
     kv8_exp<T>(sc, sl, m_run == -INFINITY ? 0.f : m_run, pb, l_run);
     __builtin_amdgcn_s_waitcnt(vmcnt_imm((NST - 1) * 2 * NI));   // V of tile t
     asm volatile("" ::: "memory");
-    const float vsc[2] = {__uint_as_float(__builtin_amdgcn_readlane(vs_l, 2 * t)),
-                          __uint_as_float(__builtin_amdgcn_readlane(vs_l, 2 * t + 1))};
+    const float vsc[2] = {__uint_as_float((uint32_t)__builtin_amdgcn_readlane(vs_l, 2 * t) << 23),
+                          __uint_as_float((uint32_t)__builtin_amdgcn_readlane(vs_l, 2 * t + 1) << 23)};
     u32x2 raw[2][NDB];
     kv8_read_v<D>(kt + Tile::kBytes, at, 0, raw);
     // (keys past the sequence's end are zeros in V)
@@ -737,24 +829,18 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
   kv8_key_range(p, s, q_first, q_last, wlo, whi);
   if (wrows == 0) whi = 0;
 
-  u32x4 qreg[2 * NDB];
-  {
-    const uint16_t* qrow = static_cast<const uint16_t*>(p.q) + kv8_base(p, s, p.q_sb, p.q_ss) +
-                           (int64_t)qi * p.q_ss + (int64_t)head * p.q_sh;
-#pragma unroll
-    for (int j = 0; j < NDB; ++j) {
-      qreg[2 * j] = load16(qrow + 32 * j + 16 * g);
-      qreg[2 * j + 1] = load16(qrow + 32 * j + 16 * g + 8);
-    }
-  }
+  Kv8Query<T, D> query;
+  query.load(static_cast<const uint16_t*>(p.q) + kv8_base(p, s, p.q_sb, p.q_ss) + (int64_t)qi * p.q_ss +
+             (int64_t)head * p.q_sh);
 
+  query.pin();
   uint8_t* ring = smem8c + kg * NST * 2 * C::kTile;
   const uint32_t ring_lds = lds_address(ring);
   int* info_page = reinterpret_cast<int*>(smem8c + C::kLds - C::kInfo);
   int* info_slot = info_page + C::kThreads;
   uint32_t* info_scale = reinterpret_cast<uint32_t*>(info_slot + C::kThreads);   // K | V << 16
 
-  const Kv8Lane<D> at;
+  const Kv8Lane<D, Kv8Query<T, D>> at;
   f32x16 acc[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) acc[db] = f32x16{};
@@ -819,8 +905,6 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
     };
 
     for (int i0 = 0; i0 < NST - 1; ++i0) issue(i0, (uint32_t)(i0 * 2 * C::kTile));
-#pragma unroll
-    for (int j = 0; j < 2 * NDB; ++j) asm volatile("" : "+v"(qreg[j]));
     if (GENERIC) asm volatile("" : "+v"(row.slope));
     uint32_t stage = 0, next_stage = (uint32_t)((NST - 1) * 2 * C::kTile);   // of tiles i0 and i0 + NST - 1
     auto advance = [](uint32_t st) { return st + 2 * C::kTile == NST * 2 * C::kTile ? 0u : st + 2 * C::kTile; };
@@ -838,16 +922,20 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
       stage = advance(stage);
       next_stage = advance(next_stage);
       if (masked.value && (t >= n_tiles || n0 >= whi || n0 + BN <= wlo)) return;
-      const float ksc[2] = {__uint_as_float((info_scale[4 * t + (c32 >> 4)] & 0xffffu) << 23),
-                            __uint_as_float((info_scale[4 * t + 2 + (c32 >> 4)] & 0xffffu) << 23)};
+      const uint32_t ksc[2] = {info_scale[4 * t + (c32 >> 4)] & 0xffffu, info_scale[4 * t + 2 + (c32 >> 4)] & 0xffffu};
       float vsc[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) vsc[u] = __uint_as_float(info_scale[4 * t + u] >> 16 << 23);
       f32x16 sc[2];
-      kv8_qk<T, F8, D, 2>(kt, at, ksc, qreg, sc);
       u32x2 raw[2][2][NDB];
-      kv8_read_v<D>(vt, at, 0, raw[0]);
-      kv8_read_v<D>(vt, at, 32, raw[1]);
+      if constexpr (D == 256) {   // (registers for the operands of 32 keys at a time)
+        query.template scores<F8, 1>(kt, at, ksc, sc);
+        query.template scores<F8, 1>(kt + 32 * D, at, ksc + 1, sc + 1);
+      } else {
+        query.template scores<F8, 2>(kt, at, ksc, sc);
+        kv8_read_v<D>(vt, at, 0, raw[0]);
+        kv8_read_v<D>(vt, at, 32, raw[1]);
+      }
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         if (GENERIC) kv8_score_options(p, row, n0 + 32 * hf, sc[hf]);
@@ -860,6 +948,7 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
       for (int hf = 0; hf < 2; ++hf) {
         u32x4 pb[2];
         kv8_exp<T>(sc[hf], sl, m_use, pb, l_run);
+        if constexpr (D == 256) kv8_read_v<D>(vt, at, 32 * hf, raw[hf]);
         kv8_pv<T, F8, D>(raw[hf], vsc + 2 * hf, pb, sc[hf], mixed, acc);
       }
     };
