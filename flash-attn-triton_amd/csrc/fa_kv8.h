@@ -54,23 +54,29 @@ struct Kv8AttnParams {
   const int* cu_q;               // packed queries: row offsets; null: [batch, seqlen_q]
   int64_t total_q;               // rows of q
   FastDiv page;
+  int first_page;                // without a table: the page of sequence 0
   int num_pages, batch, seqlen_q, heads_q, heads_k, max_keys;
   FastDiv group;
   float scale, softcap;
   const float* alibi; int64_t alibi_sb;
   int causal, window_left, window_right;
   // Launches whose sequences have at most 32 rows (queries times the group) per
-  // K/V head: kv8_split_kernel, the keys in num_splits splits of split_keys.  The
-  // others: kv8_chunk_kernel, chunk_blocks blocks of rows in all (at least).
-  // The splits of the kernel that is not launched are 0.
-  int split_keys, num_splits;
+  // K/V head: kv8_stream_kernel, `positions` equal stretches of all tiles per
+  // head (0: a workgroup per sequence).  The others (chunk_splits > 0):
+  // kv8_chunk_kernel, chunk_blocks blocks of rows in all (at least), the keys in
+  // chunk_splits splits of chunk_keys.
+  int positions, part_rows;
   int chunk_blocks, chunk_keys, chunk_splits;
-  float* o_part; float* lse_part;   // [split][row of q][head](D); LSE in log2 units
+  // Partial rows and their LSEs (log2 units): of sequence b in stretch i at
+  // [b + i][K/V head][part_rows], which no other pair of the staircase of
+  // sequences and stretches has; of splits at [split][row of q][head].
+  float* o_part; float* lse_part;
+  int* starts;   // tiles before each sequence (batch + 1), and a stretch's
 };
 
-constexpr int kKv8SplitRows = 32;
+constexpr int kKv8StreamRows = 32;
 constexpr int kKv8ChunkRows = 128;
-constexpr int kKv8MaxSplit = 4096;   // keys whose pages the lanes of a workgroup's waves hold
+constexpr int kKv8Scan = 2048;   // sequences of a kv8_stream_kernel launch, at most
 
 }  // namespace fa
 

@@ -68,28 +68,34 @@ int check_cache(const char* name, int64_t num_pages, int64_t page_size, int64_t 
 }
 
 struct Plan {
-  int split_keys, num_splits, chunk_blocks, chunk_keys, chunk_splits;
-  int64_t workspace;
+  int positions, part_rows, chunk_blocks, chunk_keys, chunk_splits;
+  int64_t each;        // sequences per launch
+  int64_t rows;        // partial rows
+  int64_t workspace;   // bytes
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Which kernel takes the launch and how the keys are split.
+// Which kernel takes the launch and how the keys are split.  No more is known
+// of the lengths than max_keys.
 Plan make_plan(int64_t batch, int64_t seqlen_q, int64_t total_q, int64_t heads_q, int64_t heads_k,
                int64_t head_dim, int64_t max_keys) {
   Plan pl = {};
   const int64_t group = heads_q / heads_k, rows = seqlen_q * group;
   max_keys = max_keys > 0 ? max_keys : 1;
-  if (rows <= fa::kKv8SplitRows) {
-    // The largest of 4096 .. 256 keys that leaves every CU several workgroups,
-    // else 128 (a tile per wave).
-    pl.split_keys = 128;
-    for (int sk = fa::kKv8MaxSplit; sk >= 256; sk /= 2)
-      if (batch * heads_k * ceil_div(max_keys, sk) >= 2048) {
-        pl.split_keys = sk;
-        break;
-      }
-    pl.num_splits = (int)ceil_div(max_keys, pl.split_keys);
+  pl.each = batch > 0 ? batch : 1;
+  if (rows <= fa::kKv8StreamRows) {
+    // A launch adds up the tiles of its sequences, in 32 bits.
+    const int64_t most = (int64_t(1) << 30) / (max_keys / 32 + 2);
+    if (pl.each > most) pl.each = most;
+    if (pl.each > fa::kKv8Scan) pl.each = fa::kKv8Scan;
+    // As many workgroups as are resident at once.  A launch of short sequences
+    // only has a workgroup for each, and no merge.
+    const int64_t slots = head_dim == 256 ? 256 : 512;
+    pl.positions = max_keys <= 512 ? 0 : (int)ceil_div(slots, heads_k);
+    pl.part_rows = (int)rows;
+    pl.rows = pl.positions > 0 ? (pl.each + pl.positions) * heads_k * rows : 0;
+    pl.workspace = pl.positions > 0 ? pl.rows * (head_dim + 1) * 4 + (pl.each + 2) * 4 : 0;
   } else {
     const int64_t most = batch * ceil_div(rows, fa::kKv8ChunkRows);
     const int64_t by_rows = total_q * group / fa::kKv8ChunkRows + batch;
@@ -100,9 +106,9 @@ Plan make_plan(int64_t batch, int64_t seqlen_q, int64_t total_q, int64_t heads_q
     n = n < cap ? n : cap;
     pl.chunk_keys = (int)(ceil_div(ceil_div(max_keys, n), 64) * 64);
     pl.chunk_splits = (int)ceil_div(max_keys, pl.chunk_keys);
+    pl.rows = pl.chunk_splits > 1 ? pl.chunk_splits * total_q * heads_q : 0;
+    pl.workspace = pl.rows * (head_dim + 1) * 4;
   }
-  const int most = pl.num_splits > pl.chunk_splits ? pl.num_splits : pl.chunk_splits;
-  pl.workspace = most > 1 ? most * total_q * heads_q * (head_dim + 1) * 4 : 0;
   return pl;
 }
 
@@ -288,6 +294,7 @@ extern "C" int fa_fwd_kvcache8(const void* q, void* out, const int64_t* q_stride
   p.total_q = total_q;
   p.page = fa::make_fastdiv((uint32_t)page_size);
   p.num_pages = (int)num_pages;
+  p.first_page = 0;
   p.batch = (int)batch;
   p.seqlen_q = (int)max_seqlen_q;
   p.heads_q = (int)heads_q;
@@ -301,15 +308,31 @@ extern "C" int fa_fwd_kvcache8(const void* q, void* out, const int64_t* q_stride
   p.causal = causal != 0;
   p.window_left = clamp_window(window_left);
   p.window_right = clamp_window(window_right);
-  p.split_keys = pl.split_keys;
-  p.num_splits = pl.num_splits;
+  p.positions = pl.positions;
+  p.part_rows = pl.part_rows;
   p.chunk_blocks = pl.chunk_blocks;
   p.chunk_keys = pl.chunk_keys;
   p.chunk_splits = pl.chunk_splits;
   p.o_part = static_cast<float*>(workspace);
-  p.lse_part = p.o_part + pl.workspace / 4 / (head_dim + 1) * head_dim;
+  p.lse_part = p.o_part + pl.rows * head_dim;
+  p.starts = reinterpret_cast<int*>(p.lse_part + pl.rows);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return hip_status(dtype == FA_DTYPE_F16 ? fa_launch_kv8_attn_f16(store, p, (int)head_dim, st)
-                                          : fa_launch_kv8_attn_bf16(store, p, (int)head_dim, st),
-                    name);
+  // (launches of a large batch follow one another in the same workspace)
+  for (int64_t b = 0; b < batch; b += pl.each) {
+    fa::Kv8AttnParams c = p;
+    c.batch = (int)(batch - b < pl.each ? batch - b : pl.each);
+    if (p.seqlens != nullptr) c.seqlens = p.seqlens + b;
+    if (p.table != nullptr) c.table = p.table + b * p.table_stride;
+    if (p.cu_q != nullptr) c.cu_q = p.cu_q + b;
+    if (p.alibi != nullptr) c.alibi = p.alibi + b * p.alibi_sb;
+    if (p.table == nullptr) c.first_page = (int)b;
+    if (p.cu_q == nullptr) {
+      c.q = static_cast<const uint16_t*>(p.q) + b * p.q_sb;
+      c.o = static_cast<uint16_t*>(p.o) + b * p.o_sb;
+    }
+    const hipError_t e = dtype == FA_DTYPE_F16 ? fa_launch_kv8_attn_f16(store, c, (int)head_dim, st)
+                                               : fa_launch_kv8_attn_bf16(store, c, (int)head_dim, st);
+    if (e != hipSuccess) return hip_status(e, name);
+  }
+  return fa_set_error(FA_OK, "");
 }

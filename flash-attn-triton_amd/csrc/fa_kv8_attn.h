@@ -2,28 +2,29 @@
 // (fa_fwd_kvcache8): one token per sequence, a few, or chunks, batched or packed.
 // The cache's layout and scales are described in fa_kv8.h.
 //
-// kv8_split_kernel.  A workgroup owns up to 32 query rows of one sequence and
-// K/V head (row r is query r / group of query head r % group, so the heads that
-// share K/V share its bytes) and a split of the keys; its four waves take
-// 32-key tiles in turn, without a barrier, and merge at the end.  The rest is
-// as in decode_kernel (fa_decode.hip): S^T = K Q^T and O^T += V^T P^T on
-// v_mfma_f32_32x32x16, one query row per lane, fp32 maximum, sum and output.
+// kv8_stream_kernel: launches of at most 32 query rows per sequence and K/V head
+// (row r is query r / group of query head r % group, so that the heads sharing
+// K/V share its bytes).  The launch is as many workgroups as fit the GPU at once,
+// and each takes an equal stretch of the sequences' 32-key tiles in a row: the
+// lengths are on the device, so every workgroup adds them up itself.  Its four
+// waves take the tiles of a sequence in turn, without a barrier, and merge; a
+// sequence within one stretch is written there, the pieces of the others are
+// merged by kv8_combine_kernel.  S^T = K Q^T and O^T += V^T P^T run on 32x32
+// matrix products, one query row per lane, with fp32 maximum, sum and output.
 // What the 8 bits change:
 //  * K and V tiles go global -> LDS as they are, by LDS-DMA into a ring of the
-//    wave's own, and become 16-bit operands on the way from LDS to the matrix
-//    core: v_cvt_scalef32_pk takes the block's power-of-two scale with it, so a
-//    key's number times its scale is exact in bf16 (and in fp16 within its
-//    range) and no score or probability is rescaled.  LDS holds and moves
-//    half of what 16-bit tiles would.
-//  * A K row is read 16 bytes at a time: lane half g gets dims 32j + 16g ..,
-//    the low 8 for product 2j and the high 8 for product 2j + 1, and Q is laid
-//    out alike.  V^T comes from ds_read_b64_tr_b8: within 16 lanes, lanes 2r
-//    and 2r + 1 name the 16 bytes of row r and lane i receives column i of the
-//    8 rows, here the 8 keys whose probabilities the lane holds.
-//  * Page numbers and scales of all of a wave's tiles are loaded at the start,
-//    one lane per 16-key group, and handed to the scalar side by v_readlane:
-//    in the loop nothing but the tile loads counts on the vector-memory
-//    counter, so each wait names the tile it needs.
+//    wave's own.  The block's power-of-two scale enters with the operand, in the
+//    scaled 8-bit product (K, bf16 queries) or in v_cvt_scalef32_pk, which makes
+//    16-bit operands (V, and K for fp16): a key's number times its scale is exact
+//    in bf16 (and in fp16 within its range), and no score or probability is
+//    rescaled.  LDS holds and moves half of what 16-bit tiles would.
+//  * V^T comes from ds_read_b64_tr_b8: within 16 lanes, lanes 2r and 2r + 1 name
+//    the 16 bytes of row r and lane i receives column i of the 8 rows, here the
+//    8 keys whose probabilities the lane holds.
+//  * Page numbers and scales of a wave's next 32 tiles are loaded together, one
+//    lane per 16-key group, and handed to the scalar side by v_readlane: in the
+//    loop nothing but the tile loads counts on the vector-memory counter, so
+//    each wait names the tile it needs.
 // Keys past the sequence's end are never read: their bytes and scales may be
 // anything.  Where the mask differs between the rows of a tile, a V number that
 // is not finite would reach rows that do not see its key (0 * NaN); such tiles
@@ -39,9 +40,8 @@
 namespace fa {
 
 constexpr int kKv8Waves = 4;
-constexpr int kKv8BN = 32;            // keys of a tile
+constexpr int kKv8BN = 32;            // keys of a tile of kv8_stream_kernel
 constexpr float kKv8Slack = 8.f;      // a maximum is raised by more than this (log2 units) or not at all
-static_assert(kKv8MaxSplit == 32 * kKv8Waves * kKv8BN, "64 lanes hold the 16-key groups of 32 tiles");
 
 // The 8-bit types.  bad(): the high bit of each byte of a word whose number is
 // not finite.
@@ -152,6 +152,14 @@ __device__ inline void kv8_key_range(const Kv8AttnParams& p, const Kv8Rows& s, i
   if (p.window_right >= 0) hi = min(hi, off + q_last + p.window_right + 1);
   if (p.window_left >= 0) lo = max(lo, off + q_first - p.window_left);
   hi = max(hi, 0);
+}
+
+// buf_load16_lds with the non-temporal hint: for data that one workgroup reads.
+__device__ inline void kv8_load_lds(const u32x4& r, uint32_t lds, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(r)
+               : "memory", "m0");
 }
 
 // What a query row of a lane sees and how its scores are scaled.
@@ -470,246 +478,322 @@ __device__ inline void kv8_raise(float mx, float& m, float& l, f32x16* acc) {
 }
 
 template <int D, int NST>
-struct Kv8Tile {
-  static constexpr int kBytes = kKv8BN * D;            // one tile of K or V
-  static constexpr int kRing = NST * 2 * kBytes;       // per wave
+struct Kv8Stream {
+  static constexpr int kTile = kKv8BN * D;             // bytes of a K or V tile
+  static constexpr int kRing = NST * 2 * kTile;        // per wave
   static constexpr int kMerge = 32 * (D + 2) * 4;      // per wave: O rows and (m, l)
-  static constexpr int kLds = kKv8Waves * (kRing > kMerge ? kRing : kMerge);
+  static constexpr int kArea = kKv8Waves * (kRing > kMerge ? kRing : kMerge);
+  static constexpr int kStarts = (kKv8Scan + 1) * 4;
+  static constexpr int kLds = kArea + kStarts;
 };
+
+// Tiles of sequence b (those that its rows see any key of).
+__device__ inline int kv8_tiles(const Kv8AttnParams& p, const Kv8Rows& s, int* first_key, int* hi) {
+  int lo;
+  kv8_key_range(p, s, 0, s.n - 1, lo, *hi);
+  *first_key = lo & ~(kKv8BN - 1);
+  return s.n > 0 && *hi > lo ? (*hi - *first_key + kKv8BN - 1) / kKv8BN : 0;
+}
+
+// starts[i] for i <= n: tiles of the launch's sequences before the i-th.
+__device__ inline void kv8_starts(const Kv8AttnParams& p, int* starts, int* wave_sum) {
+  constexpr int kPer = kKv8Scan / (kKv8Waves * 64);
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  int t[kPer], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int b = tid * kPer + i;
+    int first, hi;
+    t[i] = b < p.batch ? kv8_tiles(p, kv8_rows(p, b), &first, &hi) : 0;
+    sum += t[i];
+  }
+  int s = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int x = __shfl_up(s, d, 64);
+    if (lane >= d) s += x;
+  }
+  if (lane == 63) wave_sum[w] = s;
+  __syncthreads();
+  int before = s - sum;
+#pragma unroll
+  for (int u = 0; u < kKv8Waves; ++u)
+    if (u < w) before += wave_sum[u];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int b = tid * kPer + i;
+    if (b <= p.batch) starts[b] = before;
+    before += t[i];
+  }
+  if (tid == kKv8Waves * 64 - 1) starts[kKv8Scan] = before;
+  __syncthreads();
+}
 
 template <class T, class F8, int D, int NST, bool GENERIC>
 __global__ __launch_bounds__(kKv8Waves * 64) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
-void kv8_split_kernel(const Kv8AttnParams p) {
-  using Tile = Kv8Tile<D, NST>;
+void kv8_stream_kernel(const Kv8AttnParams p) {
+  using C = Kv8Stream<D, NST>;
   constexpr int BN = kKv8BN;
   constexpr int CPR = D / 16;              // 16-byte chunks of a row
   constexpr int RPI = 64 / CPR;            // rows of one DMA instruction
   constexpr int NI = BN / RPI;             // DMA instructions of a tile
   constexpr int IPG = 16 / RPI;            // of a 16-key group
   constexpr int NDB = D / 32;
+  constexpr int kSuper = 32 * kKv8Waves;   // tiles whose pages and scales the lanes hold
   static_assert(RPI <= 16 && 16 % RPI == 0, "an instruction stays within a 16-key group");
 
   extern __shared__ __attribute__((aligned(16))) uint8_t smem8[];
+  int* starts = reinterpret_cast<int*>(smem8 + C::kArea);
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c32 = lane & 31;
   const int g = lane >> 5;
-
-  // K/V heads vary fastest, the split slowest: as in decode_kernel.
-  int id = blockIdx.x;
-  const int kvh = id % p.heads_k;
-  id /= p.heads_k;
-  const int b = id % p.batch;
-  const int split = id / p.batch;
-
-  const Kv8Rows s = kv8_rows(p, b);
   const int G = (int)p.group.d;
-  const int rows = s.n * G;
-  if (rows <= 0 || rows > kKv8SplitRows) return;
-  int lo, hi;
-  kv8_key_range(p, s, 0, s.n - 1, lo, hi);
-  // This split's keys.  Split 0 always runs, so that rows without keys are
-  // written when there is no combine.
-  const int k_begin = max(split * p.split_keys, lo & ~(BN - 1));
-  const int k_end = min(hi, (split + 1) * p.split_keys);
-  if (k_begin >= k_end && split > 0) return;
 
-  const int r = min(c32, rows - 1);   // (lanes past the last row repeat it)
-  const bool row_valid = c32 < rows;
-  const int qi = (int)fdiv(r, p.group);
-  const int head = kvh * G + (r - qi * G);
-  const int off = p.causal ? s.L - s.n : 0;
-  Kv8Row row = kv8_row<GENERIC>(p, s, qi, head, k_end);
-  // Keys that every row sees: tiles within need no mask.
-  int all_lo = 0, all_hi = s.L - 1;
-  if (p.causal) all_hi = min(all_hi, off);
-  if (p.window_right >= 0) all_hi = min(all_hi, off + p.window_right);
-  if (p.window_left >= 0) all_lo = max(0, s.n - 1 + off - p.window_left);
-  // Q^T in the order of the K operand.
-  Kv8Query<T, D> query;
-  query.load(static_cast<const uint16_t*>(p.q) + kv8_base(p, s, p.q_sb, p.q_ss) + (int64_t)qi * p.q_ss +
-             (int64_t)head * p.q_sh);
+  // K/V heads vary fastest: the heads of a stretch of tokens run together.
+  const int kvh = blockIdx.x % p.heads_k;
+  const int pos = blockIdx.x / p.heads_k;
 
-  // Lane i holds page, slot and scales of 16-key group i % 2 of this wave's tile
-  // i / 2.  A group without keys names no page; its scale is 1.
-  const int n_tiles = k_end > k_begin ? (k_end - k_begin + BN - 1) / BN : 0;
-  const int my_tiles = (n_tiles - w + kKv8Waves - 1) / kKv8Waves;
-  int page_l = -1, slot_l = 0;
-  uint32_t ks_l = 127, vs_l = 127;   // scale bytes
-  {
-    const int key = k_begin + (w + (lane >> 1) * kKv8Waves) * BN + (lane & 1) * 16;
-    if (key < k_end) {
-      const int col = (int)fdiv(key, p.page);
-      slot_l = key - col * (int)p.page.d;
-      page_l = p.table != nullptr ? p.table[(int64_t)b * p.table_stride + col] : b;
-      if (page_l < 0 || page_l >= p.num_pages) {
-        page_l = -1;
-      } else {
-        const int blk = slot_l >> p.log2_block;
-        ks_l = p.ks[page_l * p.ks_sp + blk * p.ks_sb + kvh * p.ks_sh];
-        vs_l = p.vs[page_l * p.vs_sp + blk * p.vs_sb + kvh * p.vs_sh];
-      }
+  // This workgroup's stretch [at, stop) of the sequences' tiles in a row.
+  int b = pos, at = 0, stop = 1, per = 0;
+  if (p.positions > 0) {
+    kv8_starts(p, starts, reinterpret_cast<int*>(smem8));
+    const int total = __builtin_amdgcn_readfirstlane(starts[p.batch]);
+    per = max((total + p.positions - 1) / p.positions, kKv8Waves);
+    if (blockIdx.x == 0) {   // for the merge
+      for (int i = tid; i <= p.batch; i += kKv8Waves * 64) p.starts[i] = starts[i];
+      if (tid == 0) p.starts[p.batch + 1] = per;
     }
+    at = min(pos, total / per + 1) * per;
+    stop = min(at + per, total);
+    if (at >= stop) return;
+    b = 0;   // the last sequence that starts at or before `at`
+    for (int step = kKv8Scan / 2; step > 0; step /= 2)
+      if (b + step < p.batch && starts[b + step] <= at) b += step;
+    b = __builtin_amdgcn_readfirstlane(b);
   }
 
-  uint8_t* ring = smem8 + w * Tile::kRing;
+  const Kv8Lane<D, Kv8Query<T, D>> lane_at;
+  const float sl = GENERIC ? kLog2e : p.scale * kLog2e;
+  uint8_t* ring = smem8 + w * C::kRing;
   const uint32_t ring_lds = lds_address(ring);
-  // LDS-DMA of tile t (of this wave) into its stage.  Lane l of instruction m
-  // fills chunk position l % CPR of row m * RPI + l / CPR.
-  auto issue = [&](int t) {
-    const int key0 = k_begin + (w + t * kKv8Waves) * BN;
-    const uint32_t st = ring_lds + (uint32_t)((t % NST) * 2 * Tile::kBytes);
-    const int row_l = lane / CPR, pos = lane % CPR;
+
+  // One sequence after the other.
+  for (; at < stop; ++b) {
+    const Kv8Rows s = kv8_rows(p, b);
+    const int rows = s.n * G;
+    int first, hi;
+    const int all_tiles = kv8_tiles(p, s, &first, &hi);
+    int k_begin = first, k_end = hi, here = all_tiles;
+    if (p.positions > 0) {
+      if (all_tiles == 0) continue;
+      const int start = __builtin_amdgcn_readfirstlane(starts[b]);
+      here = min(start + all_tiles, stop) - at;
+      k_begin = first + (at - start) * BN;
+      k_end = min(hi, k_begin + here * BN);
+      at += here;
+    } else {
+      if (rows <= 0) return;
+      at = stop;
+      if (all_tiles == 0) k_end = k_begin;
+    }
+
+    const int r = min(c32, rows - 1);   // (lanes past the last row repeat it)
+    const bool row_valid = c32 < rows;
+    const int qi = (int)fdiv(r, p.group);
+    const int head = kvh * G + (r - qi * G);
+    const int off = p.causal ? s.L - s.n : 0;
+    Kv8Row row = kv8_row<GENERIC>(p, s, qi, head, k_end);
+    // Keys that every row sees: tiles within need no mask.
+    int all_lo = 0, all_hi = s.L - 1;
+    if (p.causal) all_hi = min(all_hi, off);
+    if (p.window_right >= 0) all_hi = min(all_hi, off + p.window_right);
+    if (p.window_left >= 0) all_lo = max(0, s.n - 1 + off - p.window_left);
+
+    Kv8Query<T, D> query;
+    query.load(static_cast<const uint16_t*>(p.q) + kv8_base(p, s, p.q_sb, p.q_ss) + (int64_t)qi * p.q_ss +
+               (int64_t)head * p.q_sh);
+
+    f32x16 acc[NDB];
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      const int64_t sp = kv ? p.v_sp : p.k_sp, ss = kv ? p.v_ss : p.k_ss, sh = kv ? p.v_sh : p.k_sh;
-      const uint8_t* base = kv ? p.v : p.k;
-#pragma unroll
-      for (int gr = 0; gr < 2; ++gr) {
-        // (tiles past the last get an empty resource, so that the count of
-        // loads in flight is the same on every path)
-        const int at = min(2 * t + gr, 63);
-        const int page = t < my_tiles ? __builtin_amdgcn_readlane(page_l, at) : -1;
-        const int slot = __builtin_amdgcn_readlane(slot_l, at);
-        const int left = min(s.L - (key0 + 16 * gr), 16);
-        const bool live = page >= 0 && left > 0;
-        const u32x4 rs = make_rsrc_words(live ? base + page * sp + slot * ss + kvh * sh : base,
-                                         live ? (uint32_t)((left - 1) * ss + D) : 0u);
-#pragma unroll
-        for (int m = gr * IPG; m < (gr + 1) * IPG; ++m) {
-          const int row = m * RPI + row_l;
-          const int chunk = kv ? kv8_v_chunk<D>(row, pos) : kv8_k_chunk<D>(row, pos);
-          buf_load16_lds(rs, st + (uint32_t)(kv * Tile::kBytes + m * 1024),
-                         (uint32_t)((row - 16 * gr) * (int)ss + chunk * 16));
+    for (int db = 0; db < NDB; ++db) acc[db] = f32x16{};
+    float m_run = -INFINITY, l_run = 0.f;
+    query.pin();
+
+    for (int s0 = k_begin; s0 < k_end; s0 += kSuper * BN) {
+      // Lane i holds page, slot and scale bytes of 16-key group i % 2 of this
+      // wave's tile i / 2.  A group without keys names no page; its scale is 1.
+      const int n_tiles = min((k_end - s0 + BN - 1) / BN, kSuper);
+      const int my_tiles = (n_tiles - w + kKv8Waves - 1) / kKv8Waves;
+      int page_l = -1, slot_l = 0;
+      uint32_t ks_l = 127, vs_l = 127;
+      {
+        const int key = s0 + (w + (lane >> 1) * kKv8Waves) * BN + (lane & 1) * 16;
+        if (key < k_end) {
+          const int col = (int)fdiv(key, p.page);
+          slot_l = key - col * (int)p.page.d;
+          page_l = p.table != nullptr ? p.table[(int64_t)b * p.table_stride + col] : p.first_page + b;
+          if (page_l < 0 || page_l >= p.num_pages) {
+            page_l = -1;
+          } else {
+            const int blk = slot_l >> p.log2_block;
+            ks_l = p.ks[page_l * p.ks_sp + blk * p.ks_sb + kvh * p.ks_sh];
+            vs_l = p.vs[page_l * p.vs_sp + blk * p.vs_sb + kvh * p.vs_sh];
+          }
         }
       }
-    }
-  };
 
-  const Kv8Lane<D, Kv8Query<T, D>> at;
-  f32x16 acc[NDB];
+      // LDS-DMA of tile t (of this wave) into its stage.  Lane l of instruction
+      // m fills chunk position l % CPR of row m * RPI + l / CPR.
+      auto issue = [&](int t) {
+        const int key0 = s0 + (w + t * kKv8Waves) * BN;
+        const uint32_t st = ring_lds + (uint32_t)((t % NST) * 2 * C::kTile);
+        const int row_l = lane / CPR, chunk_pos = lane % CPR;
 #pragma unroll
-  for (int db = 0; db < NDB; ++db) acc[db] = f32x16{};
-  float m_run = -INFINITY, l_run = 0.f;
-  const float sl = GENERIC ? kLog2e : p.scale * kLog2e;
+        for (int kv = 0; kv < 2; ++kv) {
+          const int64_t sp = kv ? p.v_sp : p.k_sp, ss = kv ? p.v_ss : p.k_ss, sh = kv ? p.v_sh : p.k_sh;
+          const uint8_t* base = kv ? p.v : p.k;
+#pragma unroll
+          for (int gr = 0; gr < 2; ++gr) {
+            // (tiles past the last get an empty resource, so that the count of
+            // loads in flight is the same on every path)
+            const int i = min(2 * t + gr, 63);
+            const int page = t < my_tiles ? __builtin_amdgcn_readlane(page_l, i) : -1;
+            const int slot = __builtin_amdgcn_readlane(slot_l, i);
+            const int left = min(s.L - (key0 + 16 * gr), 16);
+            const bool live = page >= 0 && left > 0;
+            const u32x4 rs = make_rsrc_words(live ? base + page * sp + slot * ss + kvh * sh : base,
+                                             live ? (uint32_t)((left - 1) * ss + D) : 0u);
+#pragma unroll
+            for (int m = gr * IPG; m < (gr + 1) * IPG; ++m) {
+              const int tr = m * RPI + row_l;
+              const int chunk = kv ? kv8_v_chunk<D>(tr, chunk_pos) : kv8_k_chunk<D>(tr, chunk_pos);
+              kv8_load_lds(rs, st + (uint32_t)(kv * C::kTile + m * 1024),
+                           (uint32_t)((tr - 16 * gr) * (int)ss + chunk * 16));
+            }
+          }
+        }
+      };
 
-  for (int t = 0; t < NST - 1; ++t) issue(t);
-  // The compiler does not count the LDS-DMA loads: a use of a loaded register
-  // inside the loop would wait there for everything in flight, so all of them
-  // are waited for here, once.
-  query.pin();
-  asm volatile("" : "+v"(ks_l), "+v"(vs_l));
-  if (GENERIC) asm volatile("" : "+v"(row.slope));
-  auto step = [&](int t, auto masked) {
-    const int n0 = k_begin + (w + t * kKv8Waves) * BN;
-    // (this wave's LDS reads of the stage that is filled now ended with the
-    // previous tile's products)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    issue(t + NST - 1);
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm((NST - 1) * 2 * NI + NI));   // K of tile t
-    asm volatile("" ::: "memory");
-    const uint8_t* kt = ring + (t % NST) * 2 * Tile::kBytes;
-    const uint32_t ks0 = __builtin_amdgcn_readlane(ks_l, 2 * t), ks1 = __builtin_amdgcn_readlane(ks_l, 2 * t + 1);
-    const uint32_t ksc = c32 < 16 ? ks0 : ks1;
-    f32x16 sc;
-    query.template scores<F8, 1>(kt, at, &ksc, &sc);
-    if (GENERIC) kv8_score_options(p, row, n0, sc);
-    if (masked.value) kv8_mask(row, n0, sc);
-    kv8_raise<NDB>(halves_max(kv8_max<1>(&sc)) * sl, m_run, l_run, acc);
-    u32x4 pb[2];
-    kv8_exp<T>(sc, sl, m_run == -INFINITY ? 0.f : m_run, pb, l_run);
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm((NST - 1) * 2 * NI));   // V of tile t
-    asm volatile("" ::: "memory");
-    const float vsc[2] = {__uint_as_float((uint32_t)__builtin_amdgcn_readlane(vs_l, 2 * t) << 23),
-                          __uint_as_float((uint32_t)__builtin_amdgcn_readlane(vs_l, 2 * t + 1) << 23)};
-    u32x2 raw[2][NDB];
-    kv8_read_v<D>(kt + Tile::kBytes, at, 0, raw);
-    // (keys past the sequence's end are zeros in V)
-    const bool mixed = masked.value && (n0 < all_lo || (n0 + BN - 1 > all_hi && all_hi < s.L - 1));
-    kv8_pv<T, F8, D>(raw, vsc, pb, sc, mixed, acc);
-  };
-  const int first = k_begin + w * BN;
-  kv8_three_runs(my_tiles, kv8_clamp(ceil_steps(all_lo - first, kKv8Waves * BN), my_tiles),
-                 kv8_clamp(ceil_steps(all_hi + 1 - BN + 1 - first, kKv8Waves * BN), my_tiles), step);
+      for (int t = 0; t < NST - 1; ++t) issue(t);
+      // The compiler does not count the LDS-DMA loads: a use of a loaded
+      // register inside the loop would wait there for everything in flight, so
+      // all of them are waited for here, once.
+      asm volatile("" : "+v"(ks_l), "+v"(vs_l));
+      if (GENERIC) asm volatile("" : "+v"(row.slope));
 
-  // ------------------------------------------------------------ merge waves
-  // The rings become the rows' merge area once every load into them has landed
-  // and every wave is done reading.
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  asm volatile("" ::: "memory");
-  __syncthreads();
-  float* mo = reinterpret_cast<float*>(smem8);
-  float* ml = mo + kKv8Waves * 32 * D;
-  const float l_w = halves_sum(l_run);
-  if (row_valid) {
-    float* orow = mo + (w * 32 + c32) * D;
-#pragma unroll
-    for (int db = 0; db < NDB; ++db)
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4)
-        *reinterpret_cast<f32x4*>(orow + db * 32 + 8 * q4 + 4 * g) =
-            f32x4{acc[db][4 * q4], acc[db][4 * q4 + 1], acc[db][4 * q4 + 2], acc[db][4 * q4 + 3]};
-    if (g == 0) {
-      ml[(w * 32 + c32) * 2] = m_run;
-      ml[(w * 32 + c32) * 2 + 1] = l_w;
+      auto step = [&](int t, auto masked) {
+        const int n0 = s0 + (w + t * kKv8Waves) * BN;
+        // (this wave's LDS reads of the stage that is filled now ended with the
+        // previous tile's products)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        issue(t + NST - 1);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((NST - 1) * 2 * NI + NI));   // K of tile t
+        asm volatile("" ::: "memory");
+        const uint8_t* kt = ring + (t % NST) * 2 * C::kTile;
+        const uint32_t ks0 = __builtin_amdgcn_readlane(ks_l, 2 * t), ks1 = __builtin_amdgcn_readlane(ks_l, 2 * t + 1);
+        const uint32_t ksc = c32 < 16 ? ks0 : ks1;
+        f32x16 sc;
+        query.template scores<F8, 1>(kt, lane_at, &ksc, &sc);
+        if (GENERIC) kv8_score_options(p, row, n0, sc);
+        if (masked.value) kv8_mask(row, n0, sc);
+        kv8_raise<NDB>(halves_max(kv8_max<1>(&sc)) * sl, m_run, l_run, acc);
+        u32x4 pb[2];
+        kv8_exp<T>(sc, sl, m_run == -INFINITY ? 0.f : m_run, pb, l_run);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((NST - 1) * 2 * NI));   // V of tile t
+        asm volatile("" ::: "memory");
+        const float vsc[2] = {__uint_as_float((uint32_t)__builtin_amdgcn_readlane(vs_l, 2 * t) << 23),
+                              __uint_as_float((uint32_t)__builtin_amdgcn_readlane(vs_l, 2 * t + 1) << 23)};
+        u32x2 raw[2][NDB];
+        kv8_read_v<D>(kt + C::kTile, lane_at, 0, raw);
+        // (keys past the sequence's end are zeros in V)
+        const bool mixed = masked.value && (n0 < all_lo || (n0 + BN - 1 > all_hi && all_hi < s.L - 1));
+        kv8_pv<T, F8, D>(raw, vsc, pb, sc, mixed, acc);
+      };
+      const int first_key = s0 + w * BN;
+      kv8_three_runs(my_tiles, kv8_clamp(ceil_steps(all_lo - first_key, kKv8Waves * BN), my_tiles),
+                     kv8_clamp(ceil_steps(min(all_hi + 1, k_end) - BN + 1 - first_key, kKv8Waves * BN), my_tiles),
+                     step);
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // (empty loads past the last tile)
+      asm volatile("" ::: "memory");
     }
-  }
-  __syncthreads();
-  // Thread t: row t / 8, D / 8 dims from D / 8 * (t % 8).
-  constexpr int DPT = D / 8;
-  const int rr = tid >> 3;
-  if (rr >= rows) return;
-  const int d0 = (tid & 7) * DPT;
-  float M = -INFINITY;
+
+    // ------------------------------------------------------------ merge waves
+    // The rings become the rows' merge area once every wave is done with them.
+    __syncthreads();
+    float* mo = reinterpret_cast<float*>(smem8);
+    float* ml = mo + kKv8Waves * 32 * D;
+    const float l_w = halves_sum(l_run);
+    if (row_valid) {
+      float* orow = mo + (w * 32 + c32) * D;
 #pragma unroll
-  for (int u = 0; u < kKv8Waves; ++u) M = fmaxf(M, ml[(u * 32 + rr) * 2]);
-  float total = 0.f, wt[kKv8Waves];
+      for (int db = 0; db < NDB; ++db)
 #pragma unroll
-  for (int u = 0; u < kKv8Waves; ++u) {
-    // (a wave without keys has l = 0; a NaN sum stays one)
-    const float l = ml[(u * 32 + rr) * 2 + 1];
-    wt[u] = l != 0.f ? __builtin_amdgcn_exp2f(ml[(u * 32 + rr) * 2] - M) : 0.f;
-    total += l * wt[u];
-  }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  float o[DPT];
-#pragma unroll
-  for (int e = 0; e < DPT; ++e) o[e] = 0.f;
-#pragma unroll
-  for (int u = 0; u < kKv8Waves; ++u) {
-    const float* src = mo + (u * 32 + rr) * D + d0;
-#pragma unroll
-    for (int e = 0; e < DPT; e += 4) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(src + e);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[e + k] = fmaf(x[k], wt[u], o[e + k]);
+        for (int q4 = 0; q4 < 4; ++q4)
+          *reinterpret_cast<f32x4*>(orow + db * 32 + 8 * q4 + 4 * g) =
+              f32x4{acc[db][4 * q4], acc[db][4 * q4 + 1], acc[db][4 * q4 + 2], acc[db][4 * q4 + 3]};
+      if (g == 0) {
+        ml[(w * 32 + c32) * 2] = m_run;
+        ml[(w * 32 + c32) * 2 + 1] = l_w;
+      }
     }
-  }
-  const int oi = (int)fdiv(rr, p.group);
-  const int oh = kvh * G + (rr - oi * G);
-  if (p.num_splits == 1) {
-    uint16_t* dst = static_cast<uint16_t*>(p.o) + kv8_base(p, s, p.o_sb, p.o_ss) +
-                    (int64_t)oi * p.o_ss + (int64_t)oh * p.o_sh + d0;
+    __syncthreads();
+    // Thread t: row t / 8, D / 8 dims from D / 8 * (t % 8).
+    constexpr int DPT = D / 8;
+    const int rr = tid >> 3;
+    if (rr < rows) {
+      const int d0 = (tid & 7) * DPT;
+      float M = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < DPT; e += 8) {
-      u32x4 val;
+      for (int u = 0; u < kKv8Waves; ++u) M = fmaxf(M, ml[(u * 32 + rr) * 2]);
+      float sum = 0.f, wt[kKv8Waves];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) val[k] = T::pack2(o[e + 2 * k] * inv, o[e + 2 * k + 1] * inv);
-      store16(dst + e, val);
+      for (int u = 0; u < kKv8Waves; ++u) {
+        // (a wave without keys has l = 0; a NaN sum stays one)
+        const float l = ml[(u * 32 + rr) * 2 + 1];
+        wt[u] = l != 0.f ? __builtin_amdgcn_exp2f(ml[(u * 32 + rr) * 2] - M) : 0.f;
+        sum += l * wt[u];
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      float o[DPT];
+#pragma unroll
+      for (int e = 0; e < DPT; ++e) o[e] = 0.f;
+#pragma unroll
+      for (int u = 0; u < kKv8Waves; ++u) {
+        const float* src = mo + (u * 32 + rr) * D + d0;
+#pragma unroll
+        for (int e = 0; e < DPT; e += 4) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(src + e);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[e + k] = fmaf(x[k], wt[u], o[e + k]);
+        }
+      }
+      if (here == all_tiles) {   // the sequence's only workgroup
+        const int oi = (int)fdiv(rr, p.group);
+        uint16_t* dst = static_cast<uint16_t*>(p.o) + kv8_base(p, s, p.o_sb, p.o_ss) + (int64_t)oi * p.o_ss +
+                        (int64_t)(kvh * G + (rr - oi * G)) * p.o_sh + d0;
+#pragma unroll
+        for (int e = 0; e < DPT; e += 8) {
+          u32x4 val;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) val[k] = T::pack2(o[e + 2 * k] * inv, o[e + 2 * k + 1] * inv);
+          store16(dst + e, val);
+        }
+      } else {
+        const int64_t prow = ((int64_t)(b + pos) * p.heads_k + kvh) * p.part_rows + rr;
+        float* dst = p.o_part + prow * D + d0;
+#pragma unroll
+        for (int e = 0; e < DPT; e += 4)
+          *reinterpret_cast<f32x4*>(dst + e) =
+              f32x4{o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
+        if ((tid & 7) == 0) p.lse_part[prow] = sum == 0.f ? -INFINITY : M + __log2f(sum);
+      }
     }
-  } else {
-    const int64_t prow = ((int64_t)split * p.total_q + kv8_out_row(p, s, oi)) * p.heads_q + oh;
-    float* dst = p.o_part + prow * D + d0;
-#pragma unroll
-    for (int e = 0; e < DPT; e += 4)
-      *reinterpret_cast<f32x4*>(dst + e) = f32x4{o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
-    if ((tid & 7) == 0)
-      p.lse_part[prow] = total == 0.f ? -INFINITY : M + __log2f(total);
+    __syncthreads();   // the next sequence's tiles come into the same LDS
   }
 }
-
 
 // kv8_chunk_kernel: launches with sequences of more than 32 query rows per K/V
 // head, and the shorter ones beside them.  A workgroup of RW x
@@ -718,7 +802,7 @@ void kv8_split_kernel(const Kv8AttnParams p) {
 // load together) and are merged at the end, so that a workgroup's chain of
 // tiles is KG times shorter: rows of long sequences beside those of short ones
 // would otherwise set the launch's time.  Tile operands, masks and scales as in
-// kv8_split_kernel; pages and scales of up to NT 16-key groups are in LDS at a time
+// kv8_stream_kernel; pages and scales of up to NT 16-key groups are in LDS at a time
 // (NT threads).
 template <int D, int RW, int KG, int NST>
 struct Kv8Chunk {
@@ -859,7 +943,7 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
       if (key < k_end) {
         const int col = (int)fdiv(key, p.page);
         slot = key - col * (int)p.page.d;
-        page = p.table != nullptr ? p.table[(int64_t)b * p.table_stride + col] : b;
+        page = p.table != nullptr ? p.table[(int64_t)b * p.table_stride + col] : p.first_page + b;
         if (page < 0 || page >= p.num_pages) {
           page = -1;
         } else {
@@ -1026,36 +1110,24 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
   }
 }
 
-// Merges the splits of four dims of a row: out = sum_s 2^(lse_s - lse) o_s over
-// the splits that hold keys its workgroup saw (the others are unwritten), the
-// partials fetched in batches of independent loads.  item: query * heads + head.
+// Merges n pieces of four dims of a row, `step` rows of the partials apart:
+// out = sum_i 2^(lse_i - lse) o_i, the partials fetched in batches of
+// independent loads.
 template <class T, int D>
-__device__ inline void kv8_combine_row(const Kv8AttnParams& p, const Kv8Rows& s, int64_t item, int qd) {
+__device__ inline void kv8_merge(const Kv8AttnParams& p, int64_t prow, int64_t step, int n, int qd, uint16_t* dst) {
   constexpr int kBatch = 8;
-  const int h = (int)(item % p.heads_q), i = (int)(item / p.heads_q);
-  const int G = (int)p.group.d;
-  // The splits that the row's workgroups ran: those that meet their keys.
-  const bool chunk = p.chunk_splits > 0;
-  const int splits = chunk ? p.chunk_splits : p.num_splits, keys = chunk ? p.chunk_keys : p.split_keys;
-  const int bm = chunk ? kKv8ChunkRows : kKv8SplitRows;
-  const int rb = (i * G + h % G) / bm, last = min(rb * bm + bm - 1, s.n * G - 1);
-  int lo, hi;
-  kv8_key_range(p, s, (int)fdiv(rb * bm, p.group), (int)fdiv(last, p.group), lo, hi);
-  const int s_lo = lo / keys;
-  const int n = hi > lo ? min(splits, (hi + keys - 1) / keys) : 0;
-  const int64_t row = kv8_out_row(p, s, i) * p.heads_q + h, step = p.total_q * p.heads_q;
   float m = -INFINITY, tot = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   bool bad = false;
-  for (int s0 = s_lo; s0 < n; s0 += kBatch) {
+  for (int i0 = 0; i0 < n; i0 += kBatch) {
     float ls[kBatch];
     f32x4 o[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const bool on = s0 + u < n;
-      ls[u] = on ? p.lse_part[(s0 + u) * step + row] : -INFINITY;
-      o[u] = on ? *reinterpret_cast<const f32x4*>(p.o_part + ((s0 + u) * step + row) * D + qd * 4)
-                : f32x4{0.f, 0.f, 0.f, 0.f};
+      const int64_t at = prow + (i0 + u) * step;
+      const bool on = i0 + u < n;
+      ls[u] = on ? p.lse_part[at] : -INFINITY;
+      o[u] = on ? *reinterpret_cast<const f32x4*>(p.o_part + at * D + qd * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
     }
     float mb = m;
 #pragma unroll
@@ -1076,54 +1148,85 @@ __device__ inline void kv8_combine_row(const Kv8AttnParams& p, const Kv8Rows& s,
     m = mb;
   }
   const float inv = bad ? __uint_as_float(0x7fc00000u) : tot > 0.f ? 1.f / tot : 0.f;
-  uint16_t* dst = static_cast<uint16_t*>(p.o) + kv8_base(p, s, p.o_sb, p.o_ss) + (int64_t)i * p.o_ss +
-                  (int64_t)h * p.o_sh + qd * 4;
   u32x2 val;
   val[0] = T::pack2(acc[0] * inv, acc[1] * inv);
   val[1] = T::pack2(acc[2] * inv, acc[3] * inv);
-  *reinterpret_cast<u32x2*>(dst) = val;
+  *reinterpret_cast<u32x2*>(dst + qd * 4) = val;
 }
 
+// The rows whose keys more than one workgroup took, and those without keys.
 // One thread per row and 4 dims, a workgroup within one sequence.
 template <class T, int D>
 __global__ __launch_bounds__(256) void kv8_combine_kernel(const Kv8AttnParams p) {
   constexpr int kQuads = D / 4;
-  const Kv8Rows s = kv8_rows(p, blockIdx.y);
+  const int b = blockIdx.y, G = (int)p.group.d;
+  const Kv8Rows s = kv8_rows(p, b);
+  int p0 = 0, pieces = 0;
+  if (p.chunk_splits == 0) {   // kv8_stream_kernel: the stretches that the sequence's tiles lie in
+    const int start = p.starts[b], end = p.starts[b + 1], per = p.starts[p.batch + 1];
+    p0 = start / per;
+    pieces = end > start ? (end - 1) / per - p0 + 1 : 0;
+    if (pieces == 1) return;
+  }
   for (int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; idx < (int64_t)s.n * p.heads_q * kQuads;
-       idx += (int64_t)gridDim.x * 256)
-    kv8_combine_row<T, D>(p, s, idx / kQuads, (int)(idx % kQuads));
+       idx += (int64_t)gridDim.x * 256) {
+    const int64_t item = idx / kQuads;
+    const int qd = (int)(idx % kQuads), h = (int)(item % p.heads_q), i = (int)(item / p.heads_q);
+    uint16_t* dst = static_cast<uint16_t*>(p.o) + kv8_base(p, s, p.o_sb, p.o_ss) + (int64_t)i * p.o_ss +
+                    (int64_t)h * p.o_sh;
+    int64_t prow, step;
+    int n = pieces;
+    if (p.chunk_splits == 0) {
+      step = (int64_t)p.heads_k * p.part_rows;
+      prow = (int64_t)(b + p0) * step + (int64_t)(h / G) * p.part_rows + i * G + h % G;
+    } else {   // kv8_chunk_kernel: the splits that meet the keys of the row's block
+      const int rb = (i * G + h % G) / kKv8ChunkRows, last = min(rb * kKv8ChunkRows + kKv8ChunkRows, s.n * G) - 1;
+      int lo, hi;
+      kv8_key_range(p, s, (int)fdiv(rb * kKv8ChunkRows, p.group), (int)fdiv(last, p.group), lo, hi);
+      const int first = lo / p.chunk_keys;
+      n = hi > lo ? min(p.chunk_splits, (hi + p.chunk_keys - 1) / p.chunk_keys) - first : 0;
+      step = p.total_q * p.heads_q;
+      prow = first * step + kv8_out_row(p, s, i) * p.heads_q + h;
+    }
+    kv8_merge<T, D>(p, prow, step, n, qd, dst);
+  }
 }
 
 template <class T, class F8, int D, bool GENERIC>
-hipError_t launch_kv8(const Kv8AttnParams& p, hipStream_t st) {
-  if (p.num_splits > 0) {
-    constexpr int NST = D == 64 ? 4 : 2;
-    using Tile = Kv8Tile<D, NST>;
-    auto kern = kv8_split_kernel<T, F8, D, NST, GENERIC>;
-    static std::atomic<uint64_t> lds_devices{0};
-    if (hipError_t e = set_lds_limit(lds_devices, kern, Tile::kLds); e != hipSuccess) return e;
-    const int64_t wgs = (int64_t)p.num_splits * p.batch * p.heads_k;
-    if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(kKv8Waves * 64), Tile::kLds, st, p);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  }
-  if (p.chunk_splits > 0) {
-    // D = 256: one wave per SIMD has the registers for a row's sums.
-    constexpr int RW = kKv8ChunkRows / 32, KG = D == 256 ? 1 : 2, NST = 3;
-    using C = Kv8Chunk<D, RW, KG, NST>;
-    auto kern = kv8_chunk_kernel<T, F8, D, RW, KG, NST, GENERIC>;
-    static std::atomic<uint64_t> lds_devices{0};
-    if (hipError_t e = set_lds_limit(lds_devices, kern, C::kLds); e != hipSuccess) return e;
-    const int64_t wgs = (int64_t)p.chunk_splits * p.chunk_blocks * p.heads_k;
-    if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(C::kThreads), C::kLds, st, p);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  }
-  if (p.num_splits <= 1 && p.chunk_splits <= 1) return hipSuccess;
+hipError_t launch_kv8_stream(Kv8AttnParams p, hipStream_t st) {
+  constexpr int NST = D == 64 ? 4 : 2;
+  using C = Kv8Stream<D, NST>;
+  auto kern = kv8_stream_kernel<T, F8, D, NST, GENERIC>;
+  static std::atomic<uint64_t> lds_devices{0};
+  if (hipError_t e = set_lds_limit(lds_devices, kern, C::kLds); e != hipSuccess) return e;
+  const int64_t wgs = (int64_t)(p.positions > 0 ? p.positions : p.batch) * p.heads_k;
+  if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(kKv8Waves * 64), C::kLds, st, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.positions == 0) return e;
+  const int64_t threads = (int64_t)p.seqlen_q * p.heads_q * (D / 4);
+  hipLaunchKernelGGL((kv8_combine_kernel<T, D>), dim3((unsigned)((threads + 255) / 256), (unsigned)p.batch),
+                     dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
+template <class T, class F8, int D, bool GENERIC>
+hipError_t launch_kv8_chunk(const Kv8AttnParams& p, hipStream_t st) {
+  // D = 256: one wave per SIMD has the registers for a row's sums.
+  constexpr int RW = kKv8ChunkRows / 32, KG = D == 256 ? 1 : 2, NST = 3;
+  using C = Kv8Chunk<D, RW, KG, NST>;
+  auto kern = kv8_chunk_kernel<T, F8, D, RW, KG, NST, GENERIC>;
+  static std::atomic<uint64_t> lds_devices{0};
+  if (hipError_t e = set_lds_limit(lds_devices, kern, C::kLds); e != hipSuccess) return e;
+  const int64_t wgs = (int64_t)p.chunk_splits * p.chunk_blocks * p.heads_k;
+  if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(C::kThreads), C::kLds, st, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.chunk_splits == 1) return e;
   // (few workgroups per sequence: most sequences of a packed batch are far
   // shorter than its longest)
-  const int64_t wgs = ((int64_t)p.seqlen_q * p.heads_q * (D / 4) + 255) / 256, cap = 8192 / p.batch + 1;
-  hipLaunchKernelGGL((kv8_combine_kernel<T, D>), dim3((unsigned)(wgs < cap ? wgs : cap), (unsigned)p.batch),
+  const int64_t most = ((int64_t)p.seqlen_q * p.heads_q * (D / 4) + 255) / 256, cap = 8192 / p.batch + 1;
+  hipLaunchKernelGGL((kv8_combine_kernel<T, D>), dim3((unsigned)(most < cap ? most : cap), (unsigned)p.batch),
                      dim3(256), 0, st, p);
   return hipGetLastError();
 }
@@ -1131,7 +1234,10 @@ hipError_t launch_kv8(const Kv8AttnParams& p, hipStream_t st) {
 template <class T>
 hipError_t launch_kv8_attn(int store, const Kv8AttnParams& p, int head_dim, hipStream_t st) {
   const bool generic = p.alibi != nullptr || p.softcap > 0.f || !(p.scale > 0.f);
-#define FA_KV8(FF, DD) return generic ? launch_kv8<T, FF, DD, true>(p, st) : launch_kv8<T, FF, DD, false>(p, st);
+#define FA_KV8(FF, DD)                                                                             \
+  if (p.chunk_splits > 0)                                                                          \
+    return generic ? launch_kv8_chunk<T, FF, DD, true>(p, st) : launch_kv8_chunk<T, FF, DD, false>(p, st); \
+  return generic ? launch_kv8_stream<T, FF, DD, true>(p, st) : launch_kv8_stream<T, FF, DD, false>(p, st);
 #define FA_KV8_D(FF)                      \
   if (head_dim == 64) { FA_KV8(FF, 64) }   \
   if (head_dim == 128) { FA_KV8(FF, 128) } \

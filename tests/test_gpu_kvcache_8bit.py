@@ -377,6 +377,58 @@ def test_decode_long(max_k):
     _check_attend([20000, 1, 0, 4095, 4097], 1, 8, 2, 128, torch.bfloat16, "e4m3", page=256, block=64, max_k=max_k)
 
 
+@pytest.mark.parametrize("batch,packed", [(70, False), (2047, False), (2050, False), (2100, True)])
+def test_decode_of_many_sequences(batch, packed):
+    # more sequences than workgroups, and than one launch adds up; some without keys or queries
+    rng = random.Random(batch)
+    lens = [rng.choice([0, 1, rng.randint(2, 90), 600 if i % 97 == 0 else 33]) for i in range(batch)]
+    counts = [rng.choice([0, 1, 2]) for _ in range(batch)] if packed else None
+    _check_attend(lens, 1, 4, 2, 64, torch.bfloat16, "e4m3", counts=counts, max_k=640 if batch > 100 else None)
+
+
+def test_decode_with_long_stretches():
+    # a workgroup takes more keys than its lanes hold pages of at a time; the pages repeat
+    st = torch.float8_e4m3fn
+    L, hk, page = 70001, 32, 64
+    kc, ks = _kv8.filled(5, page, 16, hk, 64, st, 1)
+    vc, vs = _kv8.filled(5, page, 16, hk, 64, st, 2)
+    table = torch.randint(0, 5, (1, -(-L // page)), generator=torch.Generator().manual_seed(3), dtype=torch.int32)
+    q = torch.randn(1, 1, hk, 64, generator=torch.Generator().manual_seed(4)).bfloat16()
+    want, bound = _kv8.attend(q, kc, ks, vc, vs, [L], table)
+    out = _fa().flash_attn_with_kvcache_8bit(q.to(DEV), kc.to(DEV), vc.to(DEV), ks.to(DEV), vs.to(DEV),
+                                             torch.tensor([L], device=DEV), table.to(DEV)).cpu().double()
+    assert bool(((out - want).abs() <= bound).all())
+
+
+def test_queries_of_any_size():
+    # bf16 queries are split into 8-bit numbers by their row's largest: rows of very small and large numbers, of one
+    # large number among small ones, of zeros
+    st = torch.float8_e4m3fn
+    lens = [300, 300]
+    table, pages = _table(lens, 64, 0)
+    kc, ks = _kv8.filled(pages, 64, 32, 2, 128, st, 1)
+    vc, vs = _kv8.filled(pages, 64, 32, 2, 128, st, 2)
+    q = torch.randn(2, 20, 4, 128, generator=torch.Generator().manual_seed(3))
+    q[0, 0] = 0
+    q[0, 1] *= 1e-30
+    q[0, 2, :, 5] = 3e4
+    q[0, 3, :, ::7] *= 2.0 ** -20
+    q[0, 4] *= 1e3
+    q = q.bfloat16()
+    for sq in (1, 6, 20):
+        want, bound = _kv8.attend(q[:, :sq], kc, ks, vc, vs, lens, table)
+        out = _fa().flash_attn_with_kvcache_8bit(q[:, :sq].to(DEV), kc.to(DEV), vc.to(DEV), ks.to(DEV), vs.to(DEV),
+                                                 torch.tensor(lens, device=DEV), table.to(DEV)).cpu().double()
+        assert bool(((out - want).abs() <= bound).all())
+    # a row with a number that is not finite is NaN, and it alone
+    q[0, 5, 1, 7] = math.inf
+    q[1, 2, 3, 100] = math.nan
+    out = _fa().flash_attn_with_kvcache_8bit(q.to(DEV), kc.to(DEV), vc.to(DEV), ks.to(DEV), vs.to(DEV),
+                                             torch.tensor(lens, device=DEV), table.to(DEV)).cpu()
+    nan = torch.isnan(out).all(dim=-1)
+    assert bool(nan[0, 5, 1]) and bool(nan[1, 2, 3]) and int(torch.isnan(out).any(dim=-1).sum()) == 2
+
+
 @pytest.mark.parametrize("sq", [2, 3, 8, 33, 130])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("dim", [64, 128])

@@ -129,12 +129,20 @@ def test_c_attention_checks(lib):
     assert call(batch=0, total=0) == _native.FA_OK
 
 
-def test_plan_asks_for_whole_rows(lib):
-    # fp32 rows and a sum for every split of every row of q
-    for args in ((1, 1, 1, 32, 8, 128, 131001), (64, 1, 64, 32, 8, 128, 8192), (3, 40, 50, 16, 4, 64, 4000)):
-        need = ctypes.c_int64(0)
+def test_plan_of_the_workspace(lib):
+    def plan(*args):
+        need = ctypes.c_int64(-1)
         assert lib.fa_fwd_kvcache8_plan(*args, ctypes.byref(need)) == _native.FA_OK
-        assert need.value > 0 and need.value % (args[2] * args[3] * (args[5] + 1) * 4) == 0
+        return need.value
+    # stretches of single tokens: a row per sequence and stretch, K/V head and query head, its sum, and the starts
+    assert plan(64, 1, 64, 32, 8, 128, 8192) == (64 + 64) * 32 * 129 * 4 + 66 * 4
+    # however long, and whatever the number of sequences
+    assert plan(1, 1, 1, 32, 8, 128, 1 << 20) == (1 + 64) * 32 * 129 * 4 + 3 * 4
+    assert plan(5000, 1, 5000, 32, 8, 128, 8192) == (2048 + 64) * 32 * 129 * 4 + 2050 * 4
+    assert plan(64, 1, 64, 32, 8, 128, 512) == 0
+    # chunks: whole rows of q, for each split
+    assert plan(4, 512, 2048, 32, 8, 128, 8192) == 0
+    assert plan(1, 40, 40, 16, 4, 64, 4000) % (40 * 16 * 65 * 4) == 0
 
 
 def test_scale_rule():
