@@ -76,7 +76,7 @@ struct Kv8AttnParams {
 
 constexpr int kKv8StreamRows = 32;
 constexpr int kKv8ChunkRows = 128;
-constexpr int kKv8Scan = 2048;   // sequences of a kv8_stream_kernel launch, at most
+constexpr int kKv8Scan = 256;   // sequences of a kv8_stream_kernel launch, at most
 
 }  // namespace fa
 

@@ -89,10 +89,11 @@ Plan make_plan(int64_t batch, int64_t seqlen_q, int64_t total_q, int64_t heads_q
     const int64_t most = (int64_t(1) << 30) / (max_keys / 32 + 2);
     if (pl.each > most) pl.each = most;
     if (pl.each > fa::kKv8Scan) pl.each = fa::kKv8Scan;
-    // As many workgroups as are resident at once.  A launch of short sequences
-    // only has a workgroup for each, and no merge.
+    // As many workgroups as are resident at once.  A workgroup per sequence, and
+    // no merge, where there are enough of them and none is long, or all are short.
     const int64_t slots = head_dim == 256 ? 256 : 512;
-    pl.positions = max_keys <= 512 ? 0 : (int)ceil_div(slots, heads_k);
+    const bool whole = max_keys <= 512 || (batch * heads_k >= 128 && max_keys <= 4096);
+    pl.positions = whole ? 0 : (int)ceil_div(slots, heads_k);
     pl.part_rows = (int)rows;
     pl.rows = pl.positions > 0 ? (pl.each + pl.positions) * heads_k * rows : 0;
     pl.workspace = pl.positions > 0 ? pl.rows * (head_dim + 1) * 4 + (pl.each + 2) * 4 : 0;

@@ -41,6 +41,7 @@ namespace fa {
 
 constexpr int kKv8Waves = 4;
 constexpr int kKv8BN = 32;            // keys of a tile of kv8_stream_kernel
+constexpr int kKv8Own = 32;            // tiles of the longest stretch that holds one sequence only
 constexpr float kKv8Slack = 8.f;      // a maximum is raised by more than this (log2 units) or not at all
 
 // The 8-bit types.  bad(): the high bit of each byte of a word whose number is
@@ -495,8 +496,13 @@ __device__ inline int kv8_tiles(const Kv8AttnParams& p, const Kv8Rows& s, int* f
   return s.n > 0 && *hi > lo ? (*hi - *first_key + kKv8BN - 1) / kKv8BN : 0;
 }
 
-// starts[i] for i <= n: tiles of the launch's sequences before the i-th.
-__device__ inline void kv8_starts(const Kv8AttnParams& p, int* starts, int* wave_sum) {
+// How the tiles of the launch's sequences are dealt out: starts[i] for i <= n is
+// where sequence i starts on a common axis, which stretches of the returned
+// length cut into workgroups.  Where the stretches are long, the sequences
+// follow one another, and a workgroup goes from one to the next.  Where that
+// takes longer than the tiles (a sequence costs its workgroup some 5 us before
+// and after them), each starts a stretch of its own, if there are enough.
+__device__ inline int kv8_starts(const Kv8AttnParams& p, int* starts, int* sums) {
   constexpr int kPer = kKv8Scan / (kKv8Waves * 64);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   int t[kPer], sum = 0;
@@ -507,18 +513,36 @@ __device__ inline void kv8_starts(const Kv8AttnParams& p, int* starts, int* wave
     t[i] = b < p.batch ? kv8_tiles(p, kv8_rows(p, b), &first, &hi) : 0;
     sum += t[i];
   }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
+  if (lane == 0) sums[w] = sum;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int u = 0; u < kKv8Waves; ++u) total += sums[u];
+  int per = max((total + p.positions - 1) / p.positions, kKv8Waves);
+  const int own = p.batch < p.positions
+      ? max((total + p.positions - p.batch - 1) / (p.positions - p.batch), kKv8Waves) : INT_MAX;
+  const int unit = own <= kKv8Own ? own : 1;   // sequences start at multiples of it
+  if (unit > 1) per = own;
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    t[i] = (t[i] + unit - 1) / unit * unit;
+    sum += t[i];
+  }
   int s = sum;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const int x = __shfl_up(s, d, 64);
     if (lane >= d) s += x;
   }
-  if (lane == 63) wave_sum[w] = s;
+  if (lane == 63) sums[kKv8Waves + w] = s;
   __syncthreads();
   int before = s - sum;
 #pragma unroll
   for (int u = 0; u < kKv8Waves; ++u)
-    if (u < w) before += wave_sum[u];
+    if (u < w) before += sums[kKv8Waves + u];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int b = tid * kPer + i;
@@ -527,6 +551,7 @@ __device__ inline void kv8_starts(const Kv8AttnParams& p, int* starts, int* wave
   }
   if (tid == kKv8Waves * 64 - 1) starts[kKv8Scan] = before;
   __syncthreads();
+  return __builtin_amdgcn_readfirstlane(per);
 }
 
 template <class T, class F8, int D, int NST, bool GENERIC>
@@ -559,9 +584,8 @@ void kv8_stream_kernel(const Kv8AttnParams p) {
   // This workgroup's stretch [at, stop) of the sequences' tiles in a row.
   int b = pos, at = 0, stop = 1, per = 0;
   if (p.positions > 0) {
-    kv8_starts(p, starts, reinterpret_cast<int*>(smem8));
+    per = kv8_starts(p, starts, reinterpret_cast<int*>(smem8));
     const int total = __builtin_amdgcn_readfirstlane(starts[p.batch]);
-    per = max((total + p.positions - 1) / p.positions, kKv8Waves);
     if (blockIdx.x == 0) {   // for the merge
       for (int i = tid; i <= p.batch; i += kKv8Waves * 64) p.starts[i] = starts[i];
       if (tid == 0) p.starts[p.batch + 1] = per;
@@ -591,9 +615,13 @@ void kv8_stream_kernel(const Kv8AttnParams p) {
       if (all_tiles == 0) continue;
       const int start = __builtin_amdgcn_readfirstlane(starts[b]);
       here = min(start + all_tiles, stop) - at;
+      if (here <= 0) {   // (the rest of its last stretch)
+        at = min(__builtin_amdgcn_readfirstlane(starts[b + 1]), stop);
+        continue;
+      }
       k_begin = first + (at - start) * BN;
       k_end = min(hi, k_begin + here * BN);
-      at += here;
+      at = min(__builtin_amdgcn_readfirstlane(starts[b + 1]), stop);
     } else {
       if (rows <= 0) return;
       at = stop;
@@ -620,64 +648,70 @@ void kv8_stream_kernel(const Kv8AttnParams p) {
 #pragma unroll
     for (int db = 0; db < NDB; ++db) acc[db] = f32x16{};
     float m_run = -INFINITY, l_run = 0.f;
-    query.pin();
 
-    for (int s0 = k_begin; s0 < k_end; s0 += kSuper * BN) {
-      // Lane i holds page, slot and scale bytes of 16-key group i % 2 of this
-      // wave's tile i / 2.  A group without keys names no page; its scale is 1.
-      const int n_tiles = min((k_end - s0 + BN - 1) / BN, kSuper);
-      const int my_tiles = (n_tiles - w + kKv8Waves - 1) / kKv8Waves;
-      int page_l = -1, slot_l = 0;
-      uint32_t ks_l = 127, vs_l = 127;
-      {
-        const int key = s0 + (w + (lane >> 1) * kKv8Waves) * BN + (lane & 1) * 16;
-        if (key < k_end) {
-          const int col = (int)fdiv(key, p.page);
-          slot_l = key - col * (int)p.page.d;
-          page_l = p.table != nullptr ? p.table[(int64_t)b * p.table_stride + col] : p.first_page + b;
-          if (page_l < 0 || page_l >= p.num_pages) {
-            page_l = -1;
-          } else {
-            const int blk = slot_l >> p.log2_block;
-            ks_l = p.ks[page_l * p.ks_sp + blk * p.ks_sb + kvh * p.ks_sh];
-            vs_l = p.vs[page_l * p.vs_sp + blk * p.vs_sb + kvh * p.vs_sh];
+    // Lane i holds page, slot and scale bytes of 16-key group i % 2 of this
+    // wave's tile i / 2 of the kSuper tiles from s0 on.  A group without keys names
+    // no page; its scale is 1.
+    int s0, my_tiles, page_l, slot_l;
+    uint32_t ks_l, vs_l;
+    // LDS-DMA of tile t (of this wave) into its stage.  Lane l of instruction
+    // m fills chunk position l % CPR of row m * RPI + l / CPR.
+    auto issue = [&](int t) {
+      const int key0 = s0 + (w + t * kKv8Waves) * BN;
+      const uint32_t st = ring_lds + (uint32_t)((t % NST) * 2 * C::kTile);
+      const int row_l = lane / CPR, chunk_pos = lane % CPR;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const int64_t sp = kv ? p.v_sp : p.k_sp, ss = kv ? p.v_ss : p.k_ss, sh = kv ? p.v_sh : p.k_sh;
+        const uint8_t* base = kv ? p.v : p.k;
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr) {
+          // (tiles past the last get an empty resource, so that the count of
+          // loads in flight is the same on every path)
+          const int i = min(2 * t + gr, 63);
+          const int page = t < my_tiles ? __builtin_amdgcn_readlane(page_l, i) : -1;
+          const int slot = __builtin_amdgcn_readlane(slot_l, i);
+          const int left = min(s.L - (key0 + 16 * gr), 16);
+          const bool live = page >= 0 && left > 0;
+          const u32x4 rs = make_rsrc_words(live ? base + page * sp + slot * ss + kvh * sh : base,
+                                           live ? (uint32_t)((left - 1) * ss + D) : 0u);
+#pragma unroll
+          for (int m = gr * IPG; m < (gr + 1) * IPG; ++m) {
+            const int tr = m * RPI + row_l;
+            const int chunk = kv ? kv8_v_chunk<D>(tr, chunk_pos) : kv8_k_chunk<D>(tr, chunk_pos);
+            kv8_load_lds(rs, st + (uint32_t)(kv * C::kTile + m * 1024),
+                         (uint32_t)((tr - 16 * gr) * (int)ss + chunk * 16));
           }
         }
       }
-
-      // LDS-DMA of tile t (of this wave) into its stage.  Lane l of instruction
-      // m fills chunk position l % CPR of row m * RPI + l / CPR.
-      auto issue = [&](int t) {
-        const int key0 = s0 + (w + t * kKv8Waves) * BN;
-        const uint32_t st = ring_lds + (uint32_t)((t % NST) * 2 * C::kTile);
-        const int row_l = lane / CPR, chunk_pos = lane % CPR;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const int64_t sp = kv ? p.v_sp : p.k_sp, ss = kv ? p.v_ss : p.k_ss, sh = kv ? p.v_sh : p.k_sh;
-          const uint8_t* base = kv ? p.v : p.k;
-#pragma unroll
-          for (int gr = 0; gr < 2; ++gr) {
-            // (tiles past the last get an empty resource, so that the count of
-            // loads in flight is the same on every path)
-            const int i = min(2 * t + gr, 63);
-            const int page = t < my_tiles ? __builtin_amdgcn_readlane(page_l, i) : -1;
-            const int slot = __builtin_amdgcn_readlane(slot_l, i);
-            const int left = min(s.L - (key0 + 16 * gr), 16);
-            const bool live = page >= 0 && left > 0;
-            const u32x4 rs = make_rsrc_words(live ? base + page * sp + slot * ss + kvh * sh : base,
-                                             live ? (uint32_t)((left - 1) * ss + D) : 0u);
-#pragma unroll
-            for (int m = gr * IPG; m < (gr + 1) * IPG; ++m) {
-              const int tr = m * RPI + row_l;
-              const int chunk = kv ? kv8_v_chunk<D>(tr, chunk_pos) : kv8_k_chunk<D>(tr, chunk_pos);
-              kv8_load_lds(rs, st + (uint32_t)(kv * C::kTile + m * 1024),
-                           (uint32_t)((tr - 16 * gr) * (int)ss + chunk * 16));
-            }
-          }
+    };
+    auto open = [&](int from) {
+      s0 = from;
+      my_tiles = (min((k_end - s0 + BN - 1) / BN, kSuper) - w + kKv8Waves - 1) / kKv8Waves;
+      page_l = -1;
+      slot_l = 0;
+      ks_l = vs_l = 127;
+      const int key = s0 + (w + (lane >> 1) * kKv8Waves) * BN + (lane & 1) * 16;
+      if (key < k_end) {
+        const int col = (int)fdiv(key, p.page);
+        slot_l = key - col * (int)p.page.d;
+        page_l = p.table != nullptr ? p.table[(int64_t)b * p.table_stride + col] : p.first_page + b;
+        if (page_l < 0 || page_l >= p.num_pages) {
+          page_l = -1;
+        } else {
+          const int blk = slot_l >> p.log2_block;
+          ks_l = p.ks[page_l * p.ks_sp + blk * p.ks_sb + kvh * p.ks_sh];
+          vs_l = p.vs[page_l * p.vs_sp + blk * p.vs_sb + kvh * p.vs_sh];
         }
-      };
-
+      }
       for (int t = 0; t < NST - 1; ++t) issue(t);
+    };
+
+    if (k_begin < k_end) {
+      open(k_begin);
+      query.pin();
+    }
+    while (k_begin < k_end) {
       // The compiler does not count the LDS-DMA loads: a use of a loaded
       // register inside the loop would wait there for everything in flight, so
       // all of them are waited for here, once.
@@ -718,6 +752,8 @@ void kv8_stream_kernel(const Kv8AttnParams p) {
                      step);
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // (empty loads past the last tile)
       asm volatile("" ::: "memory");
+      if (s0 + kSuper * BN >= k_end) break;
+      open(s0 + kSuper * BN);
     }
 
     // ------------------------------------------------------------ merge waves
@@ -1194,7 +1230,7 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(const Kv8AttnParams p)
 
 template <class T, class F8, int D, bool GENERIC>
 hipError_t launch_kv8_stream(Kv8AttnParams p, hipStream_t st) {
-  constexpr int NST = D == 64 ? 4 : 2;
+  constexpr int NST = D == 64 ? 3 : 2;
   using C = Kv8Stream<D, NST>;
   auto kern = kv8_stream_kernel<T, F8, D, NST, GENERIC>;
   static std::atomic<uint64_t> lds_devices{0};

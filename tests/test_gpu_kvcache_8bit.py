@@ -326,9 +326,9 @@ def _poison(kc, ks, vc, vs, lens, table, store):
 
 
 def _check_attend(lens, sq, heads, hk, dim, dtype, store, page=64, block=32, causal=True, seed=0, window=(-1, -1),
-                  softcap=0.0, alibi=False, counts=None, q_scale=1.0, poison=True, max_k=None, **kw):
+                  softcap=0.0, alibi=False, counts=None, q_scale=1.0, poison=True, max_k=None, cols_more=1, **kw):
     st = STORES[store]
-    table, pages = _table(lens, page, seed)
+    table, pages = _table(lens, page, seed, cols_more=cols_more)
     kc, ks = _kv8.filled(pages, page, block, hk, dim, st, seed + 1)
     vc, vs = _kv8.filled(pages, page, block, hk, dim, st, seed + 2)
     if poison:
@@ -356,13 +356,16 @@ def _check_attend(lens, sq, heads, hk, dim, dtype, store, page=64, block=32, cau
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("store", STORES)
 @pytest.mark.parametrize("dim", [64, 128, 256])
-def test_decode(dtype, store, dim):
-    _check_attend([1, 15, 16, 17, 31, 32, 33, 64, 65, 300, 777], 1, 8, 2, dim, dtype, store)
+@pytest.mark.parametrize("cols_more", [1, 80])
+def test_decode(dtype, store, dim, cols_more):
+    # (a table of more than 4096 keys: the sequences share workgroups)
+    _check_attend([1, 15, 16, 17, 31, 32, 33, 64, 65, 300, 777, 0, 40], 1, 8, 2, dim, dtype, store, cols_more=cols_more)
 
 
 @pytest.mark.parametrize("heads,hk", [(1, 1), (7, 1), (32, 1), (40, 1), (12, 12), (16, 8), (33, 3)])
-def test_decode_heads(heads, hk):
-    _check_attend([200, 3, 130], 1, heads, hk, 64, torch.bfloat16, "e4m3")
+@pytest.mark.parametrize("cols_more", [1, 80])
+def test_decode_heads(heads, hk, cols_more):
+    _check_attend([200, 3, 130], 1, heads, hk, 64, torch.bfloat16, "e4m3", cols_more=cols_more)
 
 
 @pytest.mark.parametrize("page,block", [(16, 16), (48, 16), (64, 64), (256, 64), (1024, 512)])
@@ -377,13 +380,13 @@ def test_decode_long(max_k):
     _check_attend([20000, 1, 0, 4095, 4097], 1, 8, 2, 128, torch.bfloat16, "e4m3", page=256, block=64, max_k=max_k)
 
 
-@pytest.mark.parametrize("batch,packed", [(70, False), (2047, False), (2050, False), (2100, True)])
+@pytest.mark.parametrize("batch,packed", [(70, False), (255, False), (256, False), (2050, False), (2100, True)])
 def test_decode_of_many_sequences(batch, packed):
     # more sequences than workgroups, and than one launch adds up; some without keys or queries
     rng = random.Random(batch)
     lens = [rng.choice([0, 1, rng.randint(2, 90), 600 if i % 97 == 0 else 33]) for i in range(batch)]
     counts = [rng.choice([0, 1, 2]) for _ in range(batch)] if packed else None
-    _check_attend(lens, 1, 4, 2, 64, torch.bfloat16, "e4m3", counts=counts, max_k=640 if batch > 100 else None)
+    _check_attend(lens, 1, 4, 2, 64, torch.bfloat16, "e4m3", counts=counts, cols_more=80)
 
 
 def test_decode_with_long_stretches():
@@ -445,7 +448,8 @@ def test_chunk_longer_than_the_cache(dim):
 @pytest.mark.parametrize("window", [(0, -1), (5, -1), (100, -1), (40, 3), (-1, 2)])
 @pytest.mark.parametrize("sq,causal", [(1, True), (6, True), (70, True), (70, False)])
 def test_windows(window, sq, causal):
-    _check_attend([sq, 100, 611], sq, 4, 2, 64, torch.bfloat16, "e4m3", window=window, causal=causal)
+    for more in (1, 80):
+        _check_attend([sq, 100, 611], sq, 4, 2, 64, torch.bfloat16, "e4m3", window=window, causal=causal, cols_more=more)
 
 
 @pytest.mark.parametrize("kind", ["alibi", "softcap", "both", "window", "scale", "zero", "negative"])

@@ -138,7 +138,7 @@ def test_plan_of_the_workspace(lib):
     assert plan(64, 1, 64, 32, 8, 128, 8192) == (64 + 64) * 32 * 129 * 4 + 66 * 4
     # however long, and whatever the number of sequences
     assert plan(1, 1, 1, 32, 8, 128, 1 << 20) == (1 + 64) * 32 * 129 * 4 + 3 * 4
-    assert plan(5000, 1, 5000, 32, 8, 128, 8192) == (2048 + 64) * 32 * 129 * 4 + 2050 * 4
+    assert plan(5000, 1, 5000, 32, 8, 128, 8192) == (256 + 64) * 32 * 129 * 4 + 258 * 4
     assert plan(64, 1, 64, 32, 8, 128, 512) == 0
     # chunks: whole rows of q, for each split
     assert plan(4, 512, 2048, 32, 8, 128, 8192) == 0
