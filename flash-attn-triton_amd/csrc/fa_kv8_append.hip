@@ -59,19 +59,25 @@ __device__ inline float scale_value(int byte) {
   return __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x00400000u);
 }
 
-// Eight numbers of a row from element d on.
+// Eight numbers of a row, as they are loaded, and in fp32.
 template <class T>
-__device__ inline void load8(const void* row, int d, float* x) {
-  if constexpr (std::is_same<T, float>::value) {
+struct Eight {
+  u32x4 w;
+  __device__ inline void load(const void* row, int d) { w = load16(static_cast<const uint16_t*>(row) + d); }
+  __device__ inline float operator[](int i) const { return T::to_float((uint16_t)(w[i / 2] >> (16 * (i & 1)))); }
+  __device__ inline void again() { asm volatile("" : "+v"(w)); }
+};
+template <>
+struct Eight<float> {
+  f32x4 w[2];
+  __device__ inline void load(const void* row, int d) {
     const f32x4* s = reinterpret_cast<const f32x4*>(static_cast<const float*>(row) + d);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = s[i / 4][i % 4];
-  } else {
-    const u32x4 w = load16(static_cast<const uint16_t*>(row) + d);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = T::to_float((uint16_t)(w[i / 2] >> (16 * (i & 1))));
+    w[0] = s[0];
+    w[1] = s[1];
   }
-}
+  __device__ inline float operator[](int i) const { return w[i / 4][i % 4]; }
+  __device__ inline void again() {}
+};
 
 }  // namespace
 
@@ -90,32 +96,40 @@ __global__ __launch_bounds__(NW * 64) void kv8_append_kernel(const Kv8AppendPara
   const int64_t x_sr = p.x_sr[t] * kBytes;
   const int block = 1 << p.log2_block;
 
-  auto usable = [&](int64_t slot) {
-    return slot >= 0 && (slot >> p.log2_block) < p.num_pages * (int64_t)p.blocks_per_page.d;
+  // What 64 rows from `row` on hold: lane i's slot, which rows begin a run and
+  // which go on with the one before (from slot to slot of a block).
+  const int64_t slots_end = (p.num_pages * (int64_t)p.blocks_per_page.d) << p.log2_block;
+  auto look = [&](int row0, int64_t* slot, uint64_t* begins, uint64_t* goes_on) {
+    const int row = row0 + lane;
+    const int64_t s = row < p.rows ? p.slots[row] : -1;
+    const int64_t before = row > 0 && row < p.rows ? p.slots[row - 1] : -1;
+    const bool usable = s >= 0 && s < slots_end;
+    const bool on = usable && before + 1 == s && (s & (block - 1)) != 0;
+    *slot = s;
+    *begins = __builtin_amdgcn_ballot_w64(usable && !on);
+    *goes_on = __builtin_amdgcn_ballot_w64(on);
   };
   const int w0 = blockIdx.x * p.window, w1 = min(w0 + p.window, p.rows);
   for (int c0 = w0; c0 < w1; c0 += 64) {
-    // Which of up to 64 rows begin a run.
-    const int row = c0 + lane;
-    bool begins = false;
-    if (row < w1) {
-      const int64_t s = p.slots[row];
-      begins = usable(s);
-      if (begins && row > 0 && (s & (block - 1)) != 0) {
-        const int64_t before = p.slots[row - 1];   // a run goes on from slot to slot of a block
-        begins = before + 1 != s;
-      }
-    }
-    for (uint64_t todo = __builtin_amdgcn_ballot_w64(begins); todo != 0; todo &= todo - 1) {
-      const int r0 = c0 + (int)__builtin_ctzll(todo);
-      const int64_t slot = p.slots[r0];
+    int64_t slot_l, unused_slot;
+    uint64_t todo, goes_on, next_goes_on, unused;
+    look(c0, &slot_l, &todo, &goes_on);
+    look(c0 + 64, &unused_slot, &unused, &next_goes_on);
+    if (w1 - c0 < 64) todo &= ((uint64_t)1 << (w1 - c0)) - 1;
+    for (; todo != 0; todo &= todo - 1) {
+      const int i0 = (int)__builtin_ctzll(todo), r0 = c0 + i0;
+      const int64_t slot =
+          (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(slot_l >> 32), i0) << 32) |
+                    (uint32_t)__builtin_amdgcn_readlane((int)slot_l, i0));
       const int first = (int)(slot & (block - 1));
-      // Rows of the run: up to the block's end, as long as the slots go on.
-      int n = min(block - first, p.rows - r0);
-      for (int i = 0; i < n; i += 64) {
-        const bool on = i + lane < n && p.slots[r0 + i + lane] == slot + i + lane;
-        const int got = __builtin_ctzll(~__builtin_amdgcn_ballot_w64(on) | 0);
-        if (~__builtin_amdgcn_ballot_w64(on) != 0) n = min(n, i + got);
+      // Rows of the run.  (The two masks hold the 64 rows behind any of the
+      // first; a larger block is looked through row group by row group.)
+      uint64_t on = goes_on >> i0 >> 1 | next_goes_on << (63 - i0);
+      int n = 1 + (on == ~(uint64_t)0 ? 64 : (int)__builtin_ctzll(~on));
+      while (n > 64 && (n - 1) % 64 == 0 && n < block - first) {
+        look(r0 + n, &unused_slot, &unused, &on);
+        n += on == ~(uint64_t)0 ? 64 : (int)__builtin_ctzll(~on);
+        if (on != ~(uint64_t)0) break;
       }
       const uint32_t gblock = (uint32_t)(slot >> p.log2_block);
       const int64_t page = fdiv(gblock, p.blocks_per_page);
@@ -126,9 +140,9 @@ __global__ __launch_bounds__(NW * 64) void kv8_append_kernel(const Kv8AppendPara
 
       // Largest finite magnitude.
       const uint8_t* xr = x + (int64_t)r0 * x_sr;
-      float keep[kKeep][8];
+      Eight<T> keep[kKeep];
       float top = 0.f;
-      auto largest = [&](const float* v) {
+      auto largest = [&](const Eight<T>& v) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float m = fabsf(v[e]);
@@ -137,16 +151,19 @@ __global__ __launch_bounds__(NW * 64) void kv8_append_kernel(const Kv8AppendPara
       };
 #pragma unroll
       for (int i = 0; i < kKeep; ++i) {
-        if (i * kRows + my_row < n) {
-          load8<T>(xr + (int64_t)(i * kRows + my_row) * x_sr, d0, keep[i]);
-          largest(keep[i]);
-        }
+        if (i * kRows + my_row < n) keep[i].load(xr + (int64_t)(i * kRows + my_row) * x_sr, d0);
       }
+#pragma unroll
+      for (int i = 0; i < kKeep; ++i)
+        if (i * kRows + my_row < n) largest(keep[i]);
       for (int i = kKeep * kRows + my_row; i < n; i += kRows) {
-        float v[8];
-        load8<T>(xr + (int64_t)i * x_sr, d0, v);
+        Eight<T> v;
+        v.load(xr + (int64_t)i * x_sr, d0);
         largest(v);
       }
+      // (as they were loaded: the compiler would keep all of them in fp32 too)
+#pragma unroll
+      for (int i = 0; i < kKeep; ++i) keep[i].again();
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
       if constexpr (NW > 1) {
@@ -160,7 +177,7 @@ __global__ __launch_bounds__(NW * 64) void kv8_append_kernel(const Kv8AppendPara
       const int need = (int)(bits >> 23) - S::kTop + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
       const int e = max(old, min(max(need, 0), 254));
 
-      auto put = [&](uint8_t* to, const float* v, float by, bool check) {
+      auto put = [&](uint8_t* to, const auto& v, float by, bool check) {
         float y[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -185,8 +202,8 @@ __global__ __launch_bounds__(NW * 64) void kv8_append_kernel(const Kv8AppendPara
       for (int i = 0; i < kKeep; ++i)
         if (i * kRows + my_row < n) put(cn + (int64_t)(i * kRows + my_row) * p.c_ss[t], keep[i], by, true);
       for (int i = kKeep * kRows + my_row; i < n; i += kRows) {
-        float v[8];
-        load8<T>(xr + (int64_t)i * x_sr, d0, v);
+        Eight<T> v;
+        v.load(xr + (int64_t)i * x_sr, d0);
         put(cn + (int64_t)i * p.c_ss[t], v, by, true);
       }
       if (tid == 0) *sp = (uint8_t)e;
