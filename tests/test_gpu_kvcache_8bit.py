@@ -60,7 +60,7 @@ def test_slots(batch, page):
     _check_slots(table, cached, added, free, page, rows)
 
 
-@pytest.mark.parametrize("batch", [2047, 2048, 2049, 5000])
+@pytest.mark.parametrize("batch", [511, 512, 513, 1100, 2047, 2048, 2049, 5000])
 def test_slots_of_many_requests(batch):
     table, cached, added, free, rows = _slots_case(batch, 16, 100, 9, batch, zero_new=True)
     _check_slots(table, cached, added, free, 16, rows, ints=torch.int64)
