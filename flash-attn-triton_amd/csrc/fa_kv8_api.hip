@@ -85,15 +85,16 @@ Plan make_plan(int64_t batch, int64_t seqlen_q, int64_t total_q, int64_t heads_q
   max_keys = max_keys > 0 ? max_keys : 1;
   pl.each = batch > 0 ? batch : 1;
   if (rows <= fa::kKv8StreamRows) {
-    // A launch adds up the tiles of its sequences, in 32 bits.
-    const int64_t most = (int64_t(1) << 30) / (max_keys / 32 + 2);
-    if (pl.each > most) pl.each = most;
-    if (pl.each > fa::kKv8Scan) pl.each = fa::kKv8Scan;
     // As many workgroups as are resident at once.  A workgroup per sequence, and
     // no merge, where there are enough of them and none is long, or all are short.
     const int64_t slots = head_dim == 256 ? 256 : 512;
     const bool whole = max_keys <= 512 || (batch * heads_k >= 128 && max_keys <= 4096);
     pl.positions = whole ? 0 : (int)ceil_div(slots, heads_k);
+    if (!whole) {   // a launch adds up the tiles of its sequences, in 32 bits
+      const int64_t most = (int64_t(1) << 30) / (max_keys / 32 + 2);
+      pl.each = pl.each < most ? pl.each : most;
+      pl.each = pl.each < fa::kKv8Scan ? pl.each : fa::kKv8Scan;
+    }
     pl.part_rows = (int)rows;
     pl.rows = pl.positions > 0 ? (pl.each + pl.positions) * heads_k * rows : 0;
     pl.workspace = pl.positions > 0 ? pl.rows * (head_dim + 1) * 4 + (pl.each + 2) * 4 : 0;
@@ -185,7 +186,7 @@ extern "C" int fa_kvcache8_append(const void* k, const void* v, const int64_t* k
   if (!head_dim_ok(head_dim))
     return fail(FA_ERR_UNSUPPORTED, "%s: head dimension must be 64, 128 or 256, not %lld", name,
                 (long long)head_dim);
-  if (tokens > kIntMax - 65536 || heads_k > 65535)
+  if (tokens > int64_t(1) << 27 || heads_k > 65535)
     return fail(FA_ERR_UNSUPPORTED, "%s: too many tokens or heads", name);
   if (tokens == 0 || num_pages == 0) return fa_set_error(FA_OK, "");
   if (k == nullptr || v == nullptr || k_cache == nullptr || v_cache == nullptr || k_scale == nullptr ||
@@ -272,8 +273,10 @@ extern "C" int fa_fwd_kvcache8(const void* q, void* out, const int64_t* q_stride
       v_cache_stride[1] > kMaxSlotStride)
     return fail(FA_ERR_UNSUPPORTED, "%s: slots that overlap or lie more than 2^26 bytes apart", name);
   const Plan pl = make_plan(batch, max_seqlen_q, total_q, heads_q, heads_k, head_dim, max_keys);
-  if (workspace_bytes < pl.workspace || (pl.workspace > 0 && workspace == nullptr))
-    return fail(FA_ERR_INVALID, "%s: the workspace must be as large as fa_fwd_kvcache8_plan says", name);
+  if (workspace_bytes < pl.workspace || (pl.workspace > 0 && workspace == nullptr) ||
+      reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return fail(FA_ERR_INVALID, "%s: the workspace must be as large as fa_fwd_kvcache8_plan says, and 16-byte aligned",
+                name);
   fa::Kv8AttnParams p;
   p.q = q;
   p.o = out;

@@ -1236,7 +1236,7 @@ hipError_t launch_kv8_stream(Kv8AttnParams p, hipStream_t st) {
   static std::atomic<uint64_t> lds_devices{0};
   if (hipError_t e = set_lds_limit(lds_devices, kern, C::kLds); e != hipSuccess) return e;
   const int64_t wgs = (int64_t)(p.positions > 0 ? p.positions : p.batch) * p.heads_k;
-  if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (wgs * kKv8Waves * 64 > 0xffffffffll) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(kKv8Waves * 64), C::kLds, st, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.positions == 0) return e;
@@ -1255,7 +1255,7 @@ hipError_t launch_kv8_chunk(const Kv8AttnParams& p, hipStream_t st) {
   static std::atomic<uint64_t> lds_devices{0};
   if (hipError_t e = set_lds_limit(lds_devices, kern, C::kLds); e != hipSuccess) return e;
   const int64_t wgs = (int64_t)p.chunk_splits * p.chunk_blocks * p.heads_k;
-  if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (wgs * C::kThreads > 0xffffffffll) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(C::kThreads), C::kLds, st, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.chunk_splits == 1) return e;

@@ -421,7 +421,7 @@ int fa_check_wait(const int64_t* result, int n, fa_stream_t stream);
  * block, heads_k]: a cached value is its number times 2^(byte - 127).  block is
  * a power of two of at least 16 that divides page_size; head_dim is 64, 128 or
  * 256.  Cache strides are {page, slot, head} in bytes, scale strides {page,
- * block, head}; rows are 16-byte aligned.  A batched cache is one whose pages
+ * block, head}; rows are 16-byte aligned, scale bytes below 255.  A batched cache is one whose pages
  * are its rows. */
 #define FA_STORE_E4M3 0
 #define FA_STORE_E5M2 1
@@ -488,8 +488,8 @@ int fa_fwd_kvcache8_plan(int64_t batch, int64_t max_seqlen_q, int64_t total_q, i
  * fa_fwd_varlen.  Rows of packed q outside every sequence are not written.
  * Whatever the device arrays hold nothing outside the tensors is read or
  * written: a page outside the cache reads as zeros, a sequence whose offsets
- * leave q has no queries.  workspace (NULL if the plan says 0) belongs to the
- * call until the stream has passed it. */
+ * leave q has no queries.  workspace (16-byte aligned; NULL if the plan
+ * says 0) belongs to the call until the stream has passed it. */
 int fa_fwd_kvcache8(const void* q, void* out, const int64_t* q_stride, const int64_t* o_stride, int dtype,
                     const void* k_cache, const void* v_cache, const int64_t* k_cache_stride,
                     const int64_t* v_cache_stride, int store, const uint8_t* k_scale,
