@@ -1151,7 +1151,7 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
 // independent loads.
 template <class T, int D>
 __device__ inline void kv8_merge(const Kv8AttnParams& p, int64_t prow, int64_t step, int n, int qd, uint16_t* dst) {
-  constexpr int kBatch = 8;
+  constexpr int kBatch = 16;
   float m = -INFINITY, tot = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   bool bad = false;

@@ -482,12 +482,14 @@ def store_code(dtype: torch.dtype) -> int:
 def kvcache_slots(block_table, cache_seqlens, new_seqlens, free_pages, free_start, page_size: int,
                   slot_mapping, positions, cu_seqlens, seqlens_out, free_end) -> None:
     """Pages and slots of the next tokens from the lengths (see fa_kvcache_slots)."""
+    batch, cols = block_table.shape
     status = load().fa_kvcache_slots(
-        _ptr(block_table), block_table.stride(0), block_table.shape[1], _ptr(cache_seqlens),
-        _ptr(new_seqlens), cache_seqlens.numel(), _ptr(free_pages), free_pages.numel(), _ptr(free_start),
-        page_size, slot_mapping.numel(), _ptr(slot_mapping), _ptr(positions), _ptr(cu_seqlens),
-        _ptr(seqlens_out), _ptr(free_end), _stream(block_table.device))
-    _check(status, "fa_kvcache_slots")
+        block_table.data_ptr(), block_table.stride(0), cols, cache_seqlens.data_ptr(), new_seqlens.data_ptr(),
+        batch, free_pages.data_ptr(), free_pages.shape[0], _ptr(free_start), page_size, slot_mapping.shape[0],
+        slot_mapping.data_ptr(), positions.data_ptr(), cu_seqlens.data_ptr(), seqlens_out.data_ptr(),
+        free_end.data_ptr(), _stream(block_table.device))
+    if status:
+        _check(status, "fa_kvcache_slots")
 
 
 def kvcache8_append(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapping) -> None:
@@ -495,12 +497,13 @@ def kvcache8_append(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapping) -> N
     T, Hk, D = k.shape
     pages, page = k_cache.shape[:2]
     status = load().fa_kvcache8_append(
-        _ptr(k), _ptr(v), _stride_array(k.stride()[:2]), _stride_array(v.stride()[:2]), dtype_code(k.dtype),
-        _ptr(k_cache), _ptr(v_cache), _stride_array(k_cache.stride()[:3]), _stride_array(v_cache.stride()[:3]),
-        store_code(k_cache.dtype), _ptr(k_scale), _ptr(v_scale), _stride_array(k_scale.stride()),
-        _stride_array(v_scale.stride()), _ptr(slot_mapping), T, pages, page, page // k_scale.shape[1], Hk, D,
+        k.data_ptr(), v.data_ptr(), _stride_array(k.stride()), _stride_array(v.stride()), dtype_code(k.dtype),
+        k_cache.data_ptr(), v_cache.data_ptr(), _stride_array(k_cache.stride()), _stride_array(v_cache.stride()),
+        store_code(k_cache.dtype), k_scale.data_ptr(), v_scale.data_ptr(), _stride_array(k_scale.stride()),
+        _stride_array(v_scale.stride()), slot_mapping.data_ptr(), T, pages, page, page // k_scale.shape[1], Hk, D,
         _stream(k.device))
-    _check(status, "fa_kvcache8_append")
+    if status:
+        _check(status, "fa_kvcache8_append")
 
 
 @functools.lru_cache(maxsize=1024)
@@ -524,20 +527,20 @@ def fwd_kvcache8(q, out, k_cache, v_cache, k_scale, v_scale, cache_seqlens, bloc
     total = q.shape[0] if packed else batch * max_seqlen_q
     ws_bytes = kvcache8_plan(batch, max_seqlen_q, total, Hq, Hk, D, max_keys)
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    qs, os_ = q.stride(), out.stride()
-    q_stride = _stride_array((0,) + qs[:2] if packed else qs[:3])
-    o_stride = _stride_array((0,) + os_[:2] if packed else os_[:3])
+    q_stride = _stride_array((0,) + q.stride() if packed else q.stride())
+    o_stride = _stride_array((0,) + out.stride() if packed else out.stride())
     tabled = block_table is not None
     status = load().fa_fwd_kvcache8(
-        _ptr(q), _ptr(out), q_stride, o_stride, dtype_code(q.dtype), _ptr(k_cache), _ptr(v_cache),
-        _stride_array(k_cache.stride()[:3]), _stride_array(v_cache.stride()[:3]), store_code(k_cache.dtype),
-        _ptr(k_scale), _ptr(v_scale), _stride_array(k_scale.stride()), _stride_array(v_scale.stride()),
+        q.data_ptr(), out.data_ptr(), q_stride, o_stride, dtype_code(q.dtype), k_cache.data_ptr(),
+        v_cache.data_ptr(), _stride_array(k_cache.stride()), _stride_array(v_cache.stride()),
+        store_code(k_cache.dtype), k_scale.data_ptr(), v_scale.data_ptr(), _stride_array(k_scale.stride()), _stride_array(v_scale.stride()),
         _ptr(cache_seqlens), _ptr(block_table), block_table.stride(0) if tabled else 0,
         block_table.shape[1] if tabled else 0, pages, page, page // k_scale.shape[1], _ptr(cu_seqlens_q),
         batch, max_seqlen_q, total, max_keys, Hq, Hk, D, softmax_scale, int(bool(causal)), window_left,
         window_right, softcap, _ptr(alibi), alibi.stride(0) if alibi is not None else 0,
         _ptr(workspace), ws_bytes, _stream(q.device))
-    _check(status, "fa_fwd_kvcache8")
+    if status:
+        _check(status, "fa_fwd_kvcache8")
 
 
 def quant_k_int8(k, k8, s_k) -> None:

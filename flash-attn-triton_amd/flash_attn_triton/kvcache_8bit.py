@@ -67,14 +67,13 @@ def _int32(t):
 
 
 def _lengths(name, t, batch, device):
-    """``t`` as one integer per sequence on ``device``."""
+    """Checks ``t``: one integer per sequence (any number of them: None) on ``device``."""
     if not isinstance(t, torch.Tensor) or t.dtype not in _INTS or t.ndim != 1:
         raise ValueError(f"{name} must be a one-dimensional int32 or int64 tensor")
     if batch is not None and t.shape[0] != batch:
         raise ValueError(f"{name} must contain one value per sequence")
     if t.device != device:
         raise ValueError(f"{name} must be on the same CUDA device")
-    return t
 
 
 def _check_cache(k_cache, v_cache, k_scale, v_scale):
