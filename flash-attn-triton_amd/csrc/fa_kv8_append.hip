@@ -19,9 +19,9 @@
 // would launch 64 empty workgroups for each that works).
 //
 // Bound: for prompts the latency of slots, then rows, then stores, covered by 16
-// waves per CU: 18800 tokens, Hk 8 D 128, bf16: 27.6 us for 115 MB (rows kept in
-// fp32 between the two sweeps, 12 waves: 45 us); for single tokens latency too: 64
-// tokens 4.4 us.
+// waves per CU: 18800 tokens, Hk 8 D 128, bf16: 27.6 us for 115 MB (with rows kept
+// in fp32 between the two sweeps, 12 waves, and the slots of a run compared one by
+// one: 38 us); for single tokens latency too: 64 tokens 4.4 us.
 #include <type_traits>
 
 #include "fa_common.h"

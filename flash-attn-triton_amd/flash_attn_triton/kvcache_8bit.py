@@ -29,6 +29,7 @@ while gradients are enabled.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -104,6 +105,29 @@ def _check_cache(k_cache, v_cache, k_scale, v_scale):
             or (ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2] | k_cache.data_ptr() | v_cache.data_ptr()) % 16):
         raise ValueError("cache rows must be contiguous and 16-byte aligned")
     return block
+
+
+@functools.lru_cache(maxsize=64)
+def _apart(shape, *strides):
+    """Whether no two elements of a tensor of ``shape`` share memory, for each of ``strides``."""
+    if 0 in shape:
+        return True
+    for stride in strides:
+        end = 0   # offset of the last element of the dimensions so far
+        for st, n in sorted((st, n) for st, n in zip(stride, shape) if n > 1):
+            if st <= end:
+                return False
+            end += st * (n - 1)
+    return True
+
+
+def _check_targets(k_cache, v_cache, k_scale, v_scale):
+    """What is written must not overlap itself: workgroups would write it at once."""
+    if k_cache.numel() and (k_cache.data_ptr() == v_cache.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr()):
+        raise ValueError("K and V must not share a cache or scales")
+    if not (_apart(k_cache.shape, k_cache.stride(), v_cache.stride())
+            and _apart(k_scale.shape, k_scale.stride(), v_scale.stride())):
+        raise ValueError("elements of the cache or its scales share memory")
 
 
 def _check_no_grad(name, *tensors):
@@ -202,7 +226,8 @@ def kvcache_append_8bit(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapping, 
     Arguments:
         k, v: (tokens, nheads_k, headdim), fp16, bf16 or fp32.
         k_cache, v_cache, k_scale, v_scale: the cache (see the module's
-            documentation), written in place.
+            documentation), written in place; no two elements may share
+            memory.
         slot_mapping: (tokens,) int64, each row's slot, page * page_size + index
             in the page, as ``paged_kvcache_slots`` gives it; a row with -1
             is skipped.
@@ -232,6 +257,7 @@ def kvcache_append_8bit(k, v, k_cache, v_cache, k_scale, v_scale, slot_mapping, 
         raise ValueError("slot_mapping must hold one int64 slot per row on the same CUDA device")
     _check_no_grad("kvcache_append_8bit", k, v)
     _check_capture(validate)
+    _check_targets(k_cache, v_cache, k_scale, v_scale)
     with _on(dev):
         slot_mapping = slot_mapping.contiguous()
         if validate and k.shape[0]:

@@ -460,7 +460,8 @@ int fa_kvcache_slots(int32_t* block_table, int64_t block_table_stride, int64_t c
  * that holds its finite numbers; another one raises it where that is needed,
  * and then rounds the slots below the run, which the block holds already, to
  * the new scale.  Rounding is to nearest even; a number that is not finite
- * becomes NaN.  Two runs of one call must not fall into the same block. */
+ * becomes NaN.  Two runs of one call must not fall into the same block, and no
+ * two elements of the caches and scales share memory. */
 int fa_kvcache8_append(const void* k, const void* v, const int64_t* k_stride, const int64_t* v_stride,
                        int dtype, void* k_cache, void* v_cache, const int64_t* k_cache_stride,
                        const int64_t* v_cache_stride, int store, uint8_t* k_scale, uint8_t* v_scale,

@@ -282,6 +282,25 @@ def test_append_of_no_rows():
                   torch.zeros(0, dtype=torch.int64))
 
 
+def test_append_refuses_targets_that_share_memory():
+    kc, ks = (t.to(DEV) for t in _kv8.filled(2, 32, 16, 2, 64, torch.float8_e4m3fn, 1))
+    vc, vs = kc.clone(), ks.clone()
+    k, slots = torch.zeros(1, 2, 64, device=DEV).half(), torch.zeros(1, dtype=torch.int64, device=DEV)
+    before = kc.cpu().view(torch.uint8).clone()
+    for cache in ((kc, kc, ks, vs), (kc, vc, ks, ks)):
+        with pytest.raises(ValueError, match="must not share"):
+            _fa().kvcache_append_8bit(k, k, *cache, slots, validate=False)
+    for cache in ((kc[:, :, :1].expand(-1, -1, 2, -1), vc, ks, vs), (kc, vc[:1].expand(2, -1, -1, -1), ks, vs),
+                  (kc, vc, ks, vs[:, :1].expand(-1, 2, -1)), (kc, vc, ks.as_strided((2, 2, 2), (4, 1, 1)), vs)):
+        with pytest.raises(ValueError, match="share memory"):
+            _fa().kvcache_append_8bit(k, k, *cache, slots, validate=False)
+    assert torch.equal(kc.cpu().view(torch.uint8), before)
+    # K and V side by side in one allocation do not
+    both = torch.stack([kc.view(torch.uint8)] * 2, dim=3).view(torch.float8_e4m3fn)
+    _fa().kvcache_append_8bit(k, k, both[:, :, :, 0], both[:, :, :, 1], ks, vs, slots)
+    assert not bool(both[0, 0].float().any()) and _kv8.same_bytes(both[0, 16:, :, 0].cpu(), kc[0, 16:].cpu())
+
+
 def test_append_refusals():
     kc, ks = (t.to(DEV) for t in _kv8.filled(2, 32, 16, 1, 64, torch.float8_e4m3fn, 1))
     k = torch.zeros(4, 1, 64, device=DEV).half()
@@ -401,6 +420,22 @@ def test_decode_with_long_stretches():
     out = _fa().flash_attn_with_kvcache_8bit(q.to(DEV), kc.to(DEV), vc.to(DEV), ks.to(DEV), vs.to(DEV),
                                              torch.tensor([L], device=DEV), table.to(DEV)).cpu().double()
     assert bool(((out - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sq", [3, 40])
+def test_query_rows_are_apart(dtype, sq):
+    # NaN and infinities in one query leave the others bit for bit as they were
+    st = torch.float8_e4m3fn
+    kc, ks = (t.to(DEV) for t in _kv8.filled(2, 256, 32, 2, 64, st, 1))
+    q = torch.randn(2, sq, 4, 64, device=DEV).to(dtype)
+    clean = _fa().flash_attn_with_kvcache_8bit(q, kc, kc, ks, ks)
+    bad = q.clone()
+    bad[0, 1, 2, 3], bad[1, 0, 0, 60] = math.nan, math.inf
+    out = _fa().flash_attn_with_kvcache_8bit(bad, kc, kc, ks, ks)
+    hit = torch.zeros(2, sq, 4, dtype=torch.bool, device=DEV)
+    hit[0, 1, 2] = hit[1, 0, 0] = True
+    assert bool(torch.isnan(out[hit]).all()) and torch.equal(out[~hit], clean[~hit])
 
 
 def test_queries_of_any_size():
@@ -555,6 +590,90 @@ def test_nan_reaches_only_rows_that_see_it(store, sq, window):
                 bad[0, i, 2:4] = True
         assert torch.equal(torch.isnan(out), bad)
         assert bool(((out - want).abs() <= bound)[~bad].all())
+
+
+def test_cache_beyond_32_bit_offsets():
+    # 5 GiB of one tensor for K and V; the sequence lies in its last pages, the append too
+    st = torch.float8_e4m3fn
+    pages, page, hk, dim = 20480, 256, 8, 128
+    big = torch.zeros(pages, page, hk, dim, dtype=torch.uint8, device=DEV).view(st)
+    scale = torch.full((pages, 4, hk), 120, dtype=torch.uint8, device=DEV).view(torch.float8_e8m0fnu)
+    kc, ks = _kv8.filled(3, page, 64, hk, dim, st, 1)
+    big.view(torch.uint8)[-3:] = kc.view(torch.uint8).to(DEV)
+    scale.view(torch.uint8)[-3:] = ks.view(torch.uint8).to(DEV)
+    table = torch.tensor([[2, 0, 1]])
+    q = torch.randn(1, 2, 16, dim, generator=torch.Generator().manual_seed(3)).bfloat16()
+    for sq in (2, 40):
+        q = torch.randn(1, sq, 16, dim, generator=torch.Generator().manual_seed(3)).bfloat16()
+        want, bound = _kv8.attend(q, kc, ks, kc, ks, [700], table, causal=True)
+        out = _fa().flash_attn_with_kvcache_8bit(q.to(DEV), big, big, scale, scale, torch.tensor([700], device=DEV),
+                                                 (table + pages - 3).to(DEV), causal=True).cpu().double()
+        assert bool(((out - want).abs() <= bound).all())
+    other, oscale = big[-3:].clone(), scale.view(torch.uint8)[-3:].clone().view(torch.float8_e8m0fnu)
+    k = _rows(300, hk, dim, torch.bfloat16, 4)
+    first = page + 188
+    slots = torch.arange(300) + first
+    wc, ws = _kv8.append(k, kc, ks, slots)
+    vbig, vscale = torch.zeros_like(big.view(torch.uint8)).view(st), scale.clone()
+    _fa().kvcache_append_8bit(k.to(DEV), k.to(DEV), big, vbig, scale, vscale, slots.to(DEV) + (pages - 3) * page)
+    assert _kv8.same_bytes(big[-3:].cpu(), wc) and torch.equal(scale[-3:].view(torch.uint8).cpu(), ws.view(torch.uint8))
+    assert not bool(big.view(torch.uint8)[:16].any())
+
+
+def test_no_visible_keys_at_all():
+    st = torch.float8_e4m3fn
+    kc, ks = (t.to(DEV) for t in _kv8.filled(3, 32, 16, 2, 64, st, 1))
+    for sq in (1, 30):
+        q = torch.randn(3, sq, 4, 64, device=DEV).half()
+        zero = torch.zeros(3, dtype=torch.int32, device=DEV)
+        for out in (_fa().flash_attn_with_kvcache_8bit(q, kc, kc, ks, ks, zero, max_seqlen_k=0),
+                    _fa().flash_attn_with_kvcache_8bit(q, kc, kc, ks, ks, zero),
+                    _fa().flash_attn_with_kvcache_8bit(q, kc[:0], kc[:0], ks[:0], ks[:0], None,
+                                                       torch.zeros(3, 200, dtype=torch.int32, device=DEV), validate=False)):
+            assert bool((out == 0).all())
+
+
+def test_capture_without_a_warm_up():
+    # the first call of its kind in the process is a captured one
+    st = torch.float8_e5m2
+    kc, ks = _kv8.filled(4, 48, 16, 3, 256, st, 1)
+    q = torch.randn(1, 1, 6, 256, generator=torch.Generator().manual_seed(3)).half()
+    want, bound = _kv8.attend(q, kc, ks, kc, ks, [150], torch.tensor([[3, 1, 0, 2]]), softcap=3.0)
+    dev = [t.to(DEV) for t in (q, kc, ks)]
+    lens, table = torch.tensor([150], dtype=torch.int32, device=DEV), torch.tensor([[3, 1, 0, 2]], dtype=torch.int32, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _fa().flash_attn_with_kvcache_8bit(dev[0], dev[1], dev[1], dev[2], dev[2], lens, table, softcap=3.0,
+                                                 validate=False)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.empty(1 << 18, device=DEV).normal_()
+        assert bool(((out.cpu().double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("causal,window,softcap", [(True, (-1, -1), 0.0), (False, (-1, -1), 0.0), (True, (9001, -1), 0.0),
+                                                   (True, (-1, -1), 9.0)])
+def test_chunk_over_more_keys_than_lds_holds_pages_of(dim, causal, window, softcap):
+    # 64 row blocks of 4 heads fill the GPU, so no block's keys are split, and one sequence has many
+    _check_attend([20011, 16384, 8193] + [33 + i for i in range(61)], 33, 4, 4, dim, torch.bfloat16, "e4m3", causal=causal,
+                  window=window, softcap=softcap)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("store", STORES)
+def test_chunks_of_256_dims(dtype, store):
+    _check_attend([70, 1, 300, 1517], 70, 6, 2, 256, dtype, store, page=48, block=16)
+    _check_attend([70, 1, 300, 1517], 70, 6, 2, 256, dtype, store, page=48, block=16, causal=False, window=(40, 30))
+
+
+def test_packed_chunks_of_many_sequences():
+    # row blocks are counted in groups of 64 sequences; some have no queries, or no keys
+    rng = random.Random(1)
+    lens = [rng.choice([0, 1, 64, rng.randint(2, 400)]) for _ in range(200)]
+    counts = [rng.choice([0, 0, 1, 7, rng.randint(2, 140)]) for _ in range(200)]
+    _check_attend(lens, 1, 4, 2, 64, torch.bfloat16, "e4m3", counts=counts)
 
 
 def test_attend_refusals():

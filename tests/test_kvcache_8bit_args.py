@@ -55,6 +55,12 @@ def test_queries_and_rows():
         kvcache_append_8bit(torch.zeros(1, 2, 64).half(), torch.zeros(1, 2, 64), *c, torch.zeros(1, dtype=torch.int64))
 
 
+def test_strides_that_share_memory():
+    from flash_attn_triton.kvcache_8bit import _apart
+    assert _apart((2, 3, 4), (12, 4, 1), (1, 8, 2), (100, 4, 1)) and _apart((1, 3, 1), (0, 1, 0)) and _apart((2, 0), (0, 1))
+    assert not _apart((2, 3, 4), (0, 4, 1)) and not _apart((2, 3, 4), (12, 3, 1)) and not _apart((2, 2), (1, 1))
+
+
 def test_slots_arguments():
     one = torch.zeros(1, dtype=torch.int32)
     with pytest.raises(ValueError, match="int32 tensor of shape"):
