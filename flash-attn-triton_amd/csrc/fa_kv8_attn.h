@@ -1154,55 +1154,60 @@ void kv8_chunk_kernel(const Kv8AttnParams p) {
   }
 }
 
-// Merges n pieces of four dims of a row, `step` rows of the partials apart:
-// out = sum_i 2^(lse_i - lse) o_i, the partials fetched in batches of
-// independent loads.
-template <class T, int D>
-__device__ inline void kv8_merge(const Kv8AttnParams& p, int64_t prow, int64_t step, int n, int qd, uint16_t* dst) {
-  constexpr int kBatch = 16;
-  float m = -INFINITY, tot = 0.f;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  bool bad = false;
-  for (int i0 = 0; i0 < n; i0 += kBatch) {
+// Four dims of a row, merged from some of its pieces.
+struct Kv8Sum {
+  float m, tot;   // largest log sum (log2 units; -inf: no keys), and the weights' sum relative to it
+  f32x4 acc;
+  bool bad;       // a log sum was NaN
+};
+
+// Merges pieces i0, i0 + SL, ... < n of four dims of a row, `step` rows of the
+// partials apart, fetched in batches of independent loads.
+template <int D, int SL>
+__device__ inline Kv8Sum kv8_merge(const Kv8AttnParams& p, int64_t prow, int64_t step, int i0, int n, int qd) {
+  constexpr int kBatch = SL > 1 ? 8 : 16;
+  Kv8Sum s = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}, false};
+  for (; i0 < n; i0 += kBatch * SL) {
     float ls[kBatch];
     f32x4 o[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int64_t at = prow + (i0 + u) * step;
-      const bool on = i0 + u < n;
+      const int64_t at = prow + (i0 + u * SL) * step;
+      const bool on = i0 + u * SL < n;
       ls[u] = on ? p.lse_part[at] : -INFINITY;
       o[u] = on ? *reinterpret_cast<const f32x4*>(p.o_part + at * D + qd * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    float mb = m;
+    float mb = s.m;
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       mb = fmaxf(mb, ls[u]);
-      bad |= ls[u] != ls[u];
+      s.bad |= ls[u] != ls[u];
     }
     if (mb == -INFINITY) continue;
-    const float again = __builtin_amdgcn_exp2f(m - mb);   // m == -inf -> 0
-    tot *= again;
-    acc *= again;
+    const float again = __builtin_amdgcn_exp2f(s.m - mb);   // m == -inf -> 0
+    s.tot *= again;
+    s.acc *= again;
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const float wgt = ls[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ls[u] - mb);
-      tot += wgt;
-      acc += wgt * o[u];
+      s.tot += wgt;
+      s.acc += wgt * o[u];
     }
-    m = mb;
+    s.m = mb;
   }
-  const float inv = bad ? __uint_as_float(0x7fc00000u) : tot > 0.f ? 1.f / tot : 0.f;
-  u32x2 val;
-  val[0] = T::pack2(acc[0] * inv, acc[1] * inv);
-  val[1] = T::pack2(acc[2] * inv, acc[3] * inv);
-  *reinterpret_cast<u32x2*>(dst + qd * 4) = val;
+  return s;
 }
 
-// The rows whose keys more than one workgroup took, and those without keys.
-// One thread per row and 4 dims, a workgroup within one sequence.
-template <class T, int D>
+// The rows whose keys more than one workgroup took, and those without keys:
+// out = sum_i 2^(lse_i - lse) o_i, a workgroup within one sequence.  A thread per
+// row and 4 dims, or, where rows have many pieces, a workgroup per row whose
+// SL slices take every SL-th piece and merge through LDS, in an order that is
+// always the same.
+template <class T, int D, int SL>
 __global__ __launch_bounds__(256) void kv8_combine_kernel(const Kv8AttnParams p) {
   constexpr int kQuads = D / 4;
+  static_assert(SL == 1 || SL * kQuads == 256, "a workgroup per row");
+  __shared__ Kv8Sum slices[SL > 1 ? 256 : 1];
   const int b = blockIdx.y, G = (int)p.group.d;
   const Kv8Rows s = kv8_rows(p, b);
   int p0 = 0, pieces = 0;
@@ -1212,8 +1217,9 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(const Kv8AttnParams p)
     pieces = end > start ? (end - 1) / per - p0 + 1 : 0;
     if (pieces == 1) return;
   }
-  for (int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; idx < (int64_t)s.n * p.heads_q * kQuads;
-       idx += (int64_t)gridDim.x * 256) {
+  const int slice = threadIdx.x / kQuads;
+  const int64_t per_wg = 256 / SL, all = (int64_t)s.n * p.heads_q * kQuads;
+  for (int64_t idx = (int64_t)blockIdx.x * per_wg + threadIdx.x % per_wg; idx < all; idx += (int64_t)gridDim.x * per_wg) {
     const int64_t item = idx / kQuads;
     const int qd = (int)(idx % kQuads), h = (int)(item % p.heads_q), i = (int)(item / p.heads_q);
     uint16_t* dst = static_cast<uint16_t*>(p.o) + kv8_base(p, s, p.o_sb, p.o_ss) + (int64_t)i * p.o_ss +
@@ -1232,8 +1238,49 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(const Kv8AttnParams p)
       step = p.total_q * p.heads_q;
       prow = first * step + kv8_out_row(p, s, i) * p.heads_q + h;
     }
-    kv8_merge<T, D>(p, prow, step, n, qd, dst);
+    Kv8Sum sum = kv8_merge<D, SL>(p, prow, step, SL > 1 ? slice : 0, n, qd);
+    if constexpr (SL > 1) {   // (one row per workgroup: every thread is here)
+      __syncthreads();        // the slices of the row before may still be read
+      slices[threadIdx.x] = sum;
+      __syncthreads();
+      if (slice > 0) continue;
+      float m = sum.m;
+#pragma unroll
+      for (int u = 1; u < SL; ++u) m = fmaxf(m, slices[u * kQuads + qd].m);
+      const float own = sum.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sum.m - m);
+      sum.tot *= own;
+      sum.acc *= own;
+#pragma unroll
+      for (int u = 1; u < SL; ++u) {
+        const Kv8Sum& t = slices[u * kQuads + qd];
+        const float wgt = t.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t.m - m);
+        sum.tot += wgt * t.tot;
+        sum.acc += wgt * t.acc;
+        sum.bad |= t.bad;
+      }
+    }
+    const float inv = sum.bad ? __uint_as_float(0x7fc00000u) : sum.tot > 0.f ? 1.f / sum.tot : 0.f;
+    *reinterpret_cast<u32x2*>(dst + qd * 4) =
+        u32x2{T::pack2(sum.acc[0] * inv, sum.acc[1] * inv), T::pack2(sum.acc[2] * inv, sum.acc[3] * inv)};
   }
+}
+
+// A workgroup merges each row where rows may have 8 pieces or more, and are few:
+// two workgroups per CU.  Decode calls with a thread per 4 dims / a workgroup per
+// row, bf16, MI355X: 32768 keys, Hq 16 Hk 1 D 128 (512 pieces) 35.7 / 18.0 us, 16
+// sequences of them (256 rows) 31.5 / 30.2; 131001 keys, Hq 32 Hk 8 D 128 (64 pieces)
+// 50.0 / 45.8; 8 sequences of 16384 (256 rows, 8 pieces) 45.9 / 45.5.  With more
+// rows a thread per 4 dims fills the GPU too: the merge alone of 1280 rows, D 64,
+// 3.8 / 6.5; calls of 2560 rows (4 chunks of 40 queries, Hq 16 Hk 4 D 128) 56.0 / 59.4.
+template <class T, int D>
+hipError_t launch_kv8_combine(const Kv8AttnParams& p, int64_t pieces, int64_t most_wgs, hipStream_t st) {
+  const int64_t rows = (int64_t)p.seqlen_q * p.heads_q, few = (rows * (D / 4) + 255) / 256;
+  const bool many = pieces >= 8 && rows * p.batch <= 512;
+  const int64_t n = many ? rows : few;
+  const dim3 grid((unsigned)(n < most_wgs ? n : most_wgs), (unsigned)p.batch);
+  if (many) hipLaunchKernelGGL((kv8_combine_kernel<T, D, 1024 / D>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((kv8_combine_kernel<T, D, 1>), grid, dim3(256), 0, st, p);
+  return hipGetLastError();
 }
 
 template <class T, class F8, int D, bool GENERIC>
@@ -1248,10 +1295,7 @@ hipError_t launch_kv8_stream(Kv8AttnParams p, hipStream_t st) {
   hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(kKv8Waves * 64), C::kLds, st, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.positions == 0) return e;
-  const int64_t threads = (int64_t)p.seqlen_q * p.heads_q * (D / 4);
-  hipLaunchKernelGGL((kv8_combine_kernel<T, D>), dim3((unsigned)((threads + 255) / 256), (unsigned)p.batch),
-                     dim3(256), 0, st, p);
-  return hipGetLastError();
+  return launch_kv8_combine<T, D>(p, p.positions / p.batch, INT_MAX, st);
 }
 
 template <class T, class F8, int D, bool GENERIC>
@@ -1269,10 +1313,7 @@ hipError_t launch_kv8_chunk(const Kv8AttnParams& p, hipStream_t st) {
   if (e != hipSuccess || p.chunk_splits == 1) return e;
   // (few workgroups per sequence: most sequences of a packed batch are far
   // shorter than its longest)
-  const int64_t most = ((int64_t)p.seqlen_q * p.heads_q * (D / 4) + 255) / 256, cap = 8192 / p.batch + 1;
-  hipLaunchKernelGGL((kv8_combine_kernel<T, D>), dim3((unsigned)(most < cap ? most : cap), (unsigned)p.batch),
-                     dim3(256), 0, st, p);
-  return hipGetLastError();
+  return launch_kv8_combine<T, D>(p, p.chunk_splits, 8192 / p.batch + 1, st);
 }
 
 template <class T>

@@ -668,6 +668,35 @@ def test_chunks_of_256_dims(dtype, store):
     _check_attend([70, 1, 300, 1517], 70, 6, 2, 256, dtype, store, page=48, block=16, causal=False, window=(40, 30))
 
 
+@pytest.mark.parametrize("heads,hk", [(3, 1), (8, 2), (32, 8), (64, 16)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[9001], [0, 5, 130, 7003], [700 * i + 1 for i in range(9)]])
+def test_merging_few_and_many_pieces(heads, hk, dim, lens):
+    # 512 pieces of a row to 2; rows of none and of one beside them
+    for sq in (1, 2):
+        _check_attend(lens, sq, heads, hk, dim, torch.bfloat16, "e4m3", seed=len(lens), cols_more=80, poison=False)
+
+
+@pytest.mark.parametrize("heads,hk,sq", [(4, 1, 33), (4, 1, 300), (12, 3, 50)])
+@pytest.mark.parametrize("lens", [[9001], [40, 5003, 0]])
+def test_merging_the_splits_of_chunks(heads, hk, sq, lens):
+    for dim in (64, 128, 256):
+        _check_attend(lens, sq, heads, hk, dim, torch.float16, "e5m2", window=(3000, -1))
+
+
+def test_nan_in_one_of_many_pieces():
+    st = torch.float8_e4m3fn
+    kc, ks = _kv8.filled(128, 64, 16, 1, 128, st, 1)
+    vc, vs = kc.clone(), ks.clone()
+    kc.view(torch.uint8)[77, 5] = 0x7f
+    q = torch.randn(1, 1, 4, 128, generator=torch.Generator().manual_seed(1)).bfloat16().to(DEV)
+    table = torch.arange(128, dtype=torch.int32, device=DEV)[None]
+    for n, bad in ((8192, True), (77 * 64 + 6, True), (77 * 64 + 5, False), (4000, False)):
+        out = _fa().flash_attn_with_kvcache_8bit(q, kc.to(DEV), vc.to(DEV), ks.to(DEV), vs.to(DEV),
+                                                 torch.tensor([n], device=DEV), table)
+        assert bool(torch.isnan(out).all()) == bad and bool(torch.isnan(out).any()) == bad
+
+
 def test_packed_chunks_of_many_sequences():
     # row blocks are counted in groups of 64 sequences; some have no queries, or no keys
     rng = random.Random(1)
